@@ -299,17 +299,73 @@ def fit(model, target, steps, lr=1e-2, graph=True, schedule=None, betas=(0.9, 0.
 class ProgressiveSplatter(nn.Module):
     """Learned feature vectors rendered through the module, coarse to fine: the image of the
     first k features must already resemble the target (the reference's
-    ``ProgressiveGaussianSplatter``, scripts/gs2d_test.py:28-51)."""
+    ``ProgressiveGaussianSplatter``, scripts/gs2d_test.py:28-51).
 
-    def __init__(self, num_features, feature_dim, gaussians_per_feature, channels=3):
+    Options beyond the reference, all off by default:
+
+    * ``tokens`` (with ``rows``): the features are not free parameters but rows of a shared
+      codebook [rows, feature_dim], feature i of image b being row ``tokens[b, i]`` times
+      ``scale``; tokens [num_features] or [B, num_features], integers.  The model then renders B
+      images at once, and a row's gradient sums over all its places.
+    * ``norm``: a layer norm with learned weight and bias on every feature vector.
+    * ``dropout``: the share of feature values that a training forward sets to zero.  Its
+      generator's state (seed, offset) is a buffer on the device that every such forward moves on
+      by one, also when a captured graph replays it.
+    """
+
+    def __init__(self, num_features, feature_dim, gaussians_per_feature, channels=3, *, tokens=None, rows=None,
+                 scale=1.0, norm=False, dropout=0.0, seed=0):
         super().__init__()
         self.num_features = int(num_features)
-        self.feature = nn.Parameter(torch.randn(1, num_features, feature_dim))
+        if (tokens is None) != (rows is None):
+            raise ValueError("tokens and rows (the codebook's size) go together")
+        if tokens is None and scale != 1.0:
+            raise ValueError("scale applies to codebook rows: it needs tokens")
+        if tokens is None:
+            self.feature = nn.Parameter(torch.randn(1, num_features, feature_dim))
+        else:
+            tokens = torch.as_tensor(tokens)
+            if tokens.dim() not in (1, 2) or tokens.shape[-1] != self.num_features or tokens.is_floating_point():
+                raise ValueError(f"tokens must be integers [{self.num_features}] or [B, {self.num_features}], got "
+                                 f"{tokens.dtype} {tuple(tokens.shape)}")
+            if tokens.numel() and not 0 <= int(tokens.min()) <= int(tokens.max()) < rows:
+                raise ValueError(f"tokens must be in 0 .. {rows - 1}")
+            self.register_buffer("tokens", tokens.to(torch.int64).reshape(-1, self.num_features))
+            self.codebook = nn.Parameter(torch.randn(int(rows), feature_dim))
+        self.scale = float(scale)
         self.gs = GaussianSplatting2D(gaussians_per_feature, feature_dim, channels)
+        self.norm_weight = nn.Parameter(torch.ones(feature_dim)) if norm else None
+        self.norm_bias = nn.Parameter(torch.zeros(feature_dim)) if norm else None
+        self.dropout = float(dropout)
+        if not 0.0 <= self.dropout < 1.0:
+            raise ValueError(f"dropout must be in 0 .. 1 (1 excluded), got {dropout}")
+        if self.dropout > 0:
+            self.register_buffer("dropout_state", torch.tensor([int(seed), 0]))
+
+    def features(self, k=None):
+        """[B,k,feature_dim]: what the renderer gets for the first k features."""
+        from . import features as ops
+
+        k = self.num_features if k is None else min(int(k), self.num_features)
+        if hasattr(self, "codebook"):
+            f = ops.embed(self.tokens[:, :k], self.codebook, scale=self.scale)
+        else:
+            f = self.feature[:, :k]
+        if self.norm_weight is not None:
+            f = ops.layer_norm(f, self.norm_weight, self.norm_bias)
+        if self.training and self.dropout > 0:
+            state = self.dropout_state.clone()  # (the backward pass reads it again)
+            self.dropout_state[1] += 1
+            f = ops.dropout(f, self.dropout, state)
+        return f
+
+    def diverse(self, k):
+        """[1,N,feature_dim]: the learned vectors that the diversity term of ``fit_progressive``
+        spreads, the first k features or the codebook's rows."""
+        return self.codebook[None] if hasattr(self, "codebook") else self.feature[:, :k]
 
     def forward(self, num_active_features=None, size=None):
-        k = self.num_features if num_active_features is None else min(int(num_active_features), self.num_features)
-        return self.gs(self.feature[:, :k], size)
+        return self.gs(self.features(num_active_features), size)
 
 
 def fit_progressive(model, target, steps, lr=1e-4, chunk=4, ratios=(1 / 16, 1 / 8, 1 / 4, 1 / 2, 1.0),
@@ -317,7 +373,8 @@ def fit_progressive(model, target, steps, lr=1e-4, chunk=4, ratios=(1 / 16, 1 / 
     """The training loop of the reference's feature -> image experiment
     (scripts/gs2d_test.py:154-189): every step draws a fraction of the features, renders
     only those, and steps AdamW on ``reconstruction + reg_weight * koleo(features[:k])``
-    with the gradient norm clipped to ``clip``.  The reconstruction term is L1 + 0.5 MSE
+    (of the codebook's rows for a model with tokens) with the gradient norm clipped to
+    ``clip``.  The reconstruction term is L1 + 0.5 MSE
     (:53-60 without its MS-SSIM term, whose package is not available here).  Returns
     (losses [steps], the k of every step) on the CPU."""
     from .reg import koleo_diversity_loss
@@ -337,7 +394,7 @@ def fit_progressive(model, target, steps, lr=1e-4, chunk=4, ratios=(1 / 16, 1 / 
         ks.append(k)
         out, _ = model(num_active_features=k, size=size)
         recon = F.l1_loss(out, target) + 0.5 * mse_loss(out, target)
-        loss = recon + reg_weight * koleo_diversity_loss(model.feature[:, :k])
+        loss = recon + reg_weight * koleo_diversity_loss(model.diverse(k))
         opt.zero_grad(set_to_none=True)
         loss.backward()
         torch.nn.utils.clip_grad_norm_(model.parameters(), clip)

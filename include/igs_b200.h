@@ -390,6 +390,76 @@ int igs_profile_enable(int on);
 int igs_profile_reset(void);
 int igs_profile_read(int kernel_id, double* total_ms, long long* launches);
 
+/*
+ * Feature operators: what stands between an image's tokens and the feature vectors that
+ * igs_forward_feature's projection starts from.  No counterpart in the reference, whose
+ * features are free parameters (scripts/gs2d_test.py:28-51): additions of this library.
+ *
+ * Tensors are of one of three types, computed in 32 bits and rounded once; the codes:
+ */
+#define IGS_F32 0
+#define IGS_BF16 1
+#define IGS_F16 2
+
+/*
+ * Embedding lookup.  out [n,D] = scale * table[tokens[i]]; tokens int32 (token_bytes 4) or
+ * int64 (8), table [rows,D] with `row_stride` elements from one row to the next (inner stride
+ * 1), out contiguous and of the table's type.
+ *   has_empty / empty: a token that marks a place without one; its row is zero;
+ *   any other token outside 0 .. rows-1 reads nothing and gives a row of NaN.
+ * Limits: n <= 2^31 - 2^20, rows <= 2^31 - 2, D <= 2^22 (else IGS_ERR_LIMIT).
+ */
+int igs_embed(const void* tokens, int token_bytes, long long n, const void* table, int dtype,
+              long long rows, long long D, long long row_stride, float scale, int has_empty,
+              long long empty, void* out, int device, void* stream);
+
+/*
+ * The table's gradient, by sorted tokens: d_table [rows,D] (contiguous, of dy's type) =
+ * scale * the sum of dy's rows [n,D] (contiguous) over the places of each token, zero for rows
+ * without one.  Every row is written.  Empty places and tokens outside the table add nothing.
+ * No floating-point atomics: the same bits on every call.
+ */
+int igs_embed_grad_workspace_bytes(long long n, long long rows, long long D, int device, size_t* bytes);
+int igs_embed_grad(const void* tokens, int token_bytes, long long n, const void* dy, int dtype,
+                   long long rows, long long D, float scale, int has_empty, long long empty,
+                   void* d_table, void* workspace, size_t workspace_bytes, int device, void* stream);
+
+/*
+ * Layer norm over rows of D values: y = (x - mean) * rstd * weight + bias, rstd =
+ * 1 / sqrt(var + eps) with the biased variance.  x [rows,D] with `row_stride` elements between
+ * rows, y [rows,D] contiguous; weight, bias [D] of type wdtype (x's type or IGS_F32) or NULL
+ * for ones / zeros.  shift, rstd [rows] (fp32) are what the gradient needs; both NULL when it is
+ * not wanted.  The mean is kept as its distance from the row's first value, mean = x[0] + shift,
+ * so that rows far from zero lose nothing.
+ */
+int igs_layer_norm(const void* x, int dtype, long long rows, long long D, long long row_stride,
+                   const void* weight, const void* bias, int wdtype, float eps, void* y, float* shift,
+                   float* rstd, int device, void* stream);
+
+/*
+ * Its gradient: dx [rows,D] (contiguous, x's type), dweight and dbias [D] (wdtype), each NULL
+ * when not wanted.  dy [rows,D] contiguous.  The column sums are taken over fixed blocks of
+ * rows and added in a fixed order: the same bits on every call.
+ */
+size_t igs_layer_norm_grad_workspace_bytes(long long rows, long long D);
+int igs_layer_norm_grad(const void* dy, const void* x, int dtype, long long rows, long long D,
+                        long long row_stride, const void* weight, int wdtype, const float* shift,
+                        const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                        size_t workspace_bytes, int device, void* stream);
+
+/*
+ * Dropout: y[i] = x[i] / (1 - p) where the generator keeps value i, 0 where it does not
+ * (whatever x[i] is), i over n contiguous values.  The generator is Philox4x32 with 7 rounds:
+ * value i takes word i % 4 of the block with counter (i / 4, offset) and key seed, and is kept
+ * when the word is at least floor(p * 2^32).  The mask is stored nowhere: the gradient is the
+ * same call on the upstream gradient.
+ *   state: NULL, or two int64 (seed, offset) on the device, read when the kernel runs (a
+ *   captured graph then draws a new mask per replay if the state changes in between): its seed
+ *   replaces `seed`, its offset is added to `offset`.  y may be x.
+ */
+int igs_dropout(const void* x, int dtype, long long n, double p, unsigned long long seed,
+                unsigned long long offset, const long long* state, void* y, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
