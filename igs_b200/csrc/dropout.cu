@@ -12,6 +12,7 @@ namespace igs {
 
 constexpr int PHILOX_ROUNDS = 7;
 constexpr int DROPOUT_THREADS = 256;
+constexpr long long DROPOUT_MAX = 1ll << 42;  // values a call takes: the grid stays within 2^31 - 1 blocks
 
 struct PhiloxKeys {
     uint32_t k0[PHILOX_ROUNDS], k1[PHILOX_ROUNDS];
@@ -56,8 +57,16 @@ struct DropoutArgs {
     float scale;             // 1 / (1 - p)
 };
 
-// One thread per four neighbouring values: one generator block.
 template <typename T>
+__device__ __forceinline__ T dropped(T x, uint32_t word, const DropoutArgs& a) {
+    return word >= a.threshold ? from_f<T>(to_f(x) * a.scale) : from_f<T>(0.f);
+}
+
+// A thread takes DROPOUT_UNROLL groups of V neighbouring values, all loads first; V is 16 bytes'
+// worth (one or two generator blocks) or, where x or y is off the 16-byte boundary, four values
+// moved one by one.  The last n % V values go to the last block's first threads.
+constexpr int DROPOUT_UNROLL = 4;
+template <typename T, int V, bool ALIGNED>
 __global__ void __launch_bounds__(DROPOUT_THREADS) dropout_kernel(DropoutArgs a) {
     unsigned long long seed = a.seed, offset = a.offset;
     if (a.state) {
@@ -67,15 +76,45 @@ __global__ void __launch_bounds__(DROPOUT_THREADS) dropout_kernel(DropoutArgs a)
     const PhiloxKeys keys = philox_keys(seed, offset);
     const T* x = static_cast<const T*>(a.x);
     T* y = static_cast<T*>(a.y);
-    const long long blocks = (a.n + 3) / 4, step = (long long)gridDim.x * DROPOUT_THREADS;
-    for (long long q = (long long)blockIdx.x * DROPOUT_THREADS + threadIdx.x; q < blocks; q += step) {
-        const uint4 r = philox(keys, (unsigned long long)q);
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    const long long groups = a.n / V;
+    const long long g0 = (long long)blockIdx.x * (DROPOUT_THREADS * DROPOUT_UNROLL) + threadIdx.x;
+    Pack<T, V> in[DROPOUT_UNROLL];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const long long i = q * 4 + j;
-            if (i < a.n) y[i] = w[j] >= a.threshold ? from_f<T>(to_f(x[i]) * a.scale) : from_f<T>(0.f);
+    for (int u = 0; u < DROPOUT_UNROLL; ++u) {
+        const long long g = g0 + u * DROPOUT_THREADS;
+        if (g >= groups) continue;
+        if constexpr (ALIGNED) {
+            in[u] = reinterpret_cast<const Pack<T, V>*>(x)[g];
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) in[u].v[j] = x[g * V + j];
         }
+    }
+#pragma unroll
+    for (int u = 0; u < DROPOUT_UNROLL; ++u) {
+        const long long g = g0 + u * DROPOUT_THREADS;
+        if (g >= groups) continue;
+        Pack<T, V> out;
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+            const uint4 r = philox(keys, (unsigned long long)(g * (V / 4) + q));
+            out.v[4 * q] = dropped(in[u].v[4 * q], r.x, a);
+            out.v[4 * q + 1] = dropped(in[u].v[4 * q + 1], r.y, a);
+            out.v[4 * q + 2] = dropped(in[u].v[4 * q + 2], r.z, a);
+            out.v[4 * q + 3] = dropped(in[u].v[4 * q + 3], r.w, a);
+        }
+        if constexpr (ALIGNED) {
+            reinterpret_cast<Pack<T, V>*>(y)[g] = out;
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) y[g * V + j] = out.v[j];
+        }
+    }
+    const long long i = groups * V + threadIdx.x;
+    if (blockIdx.x == gridDim.x - 1 && i < a.n) {
+        const uint4 r = philox(keys, (unsigned long long)(i / 4));
+        const uint32_t w = i % 4 == 0 ? r.x : i % 4 == 1 ? r.y : i % 4 == 2 ? r.z : r.w;
+        y[i] = dropped(x[i], w, a);
     }
 }
 
@@ -86,6 +125,7 @@ using namespace igs;
 extern "C" int igs_dropout(const void* x, int dtype, long long n, double p, unsigned long long seed,
                            unsigned long long offset, const long long* state, void* y, int device, void* stream) {
     if (n < 0 || !dtype_ok(dtype) || !(p >= 0.0 && p <= 1.0)) return IGS_ERR_ARG;
+    if (n > DROPOUT_MAX) return IGS_ERR_LIMIT;
     if (n == 0) return IGS_OK;
     if (!x || !y) return IGS_ERR_ARG;
     DeviceGuard guard(device);
@@ -95,11 +135,16 @@ extern "C" int igs_dropout(const void* x, int dtype, long long n, double p, unsi
         return (int)cudaMemsetAsync(y, 0, (size_t)n * dtype_size(dtype), s);
 
     DropoutArgs a{x, y, n, seed, offset, state, (uint32_t)(p * 4294967296.0), (float)(1.0 / (1.0 - p))};
-    const long long want = ((n + 3) / 4 + DROPOUT_THREADS - 1) / DROPOUT_THREADS;
-    const long long most = (long long)sm_count(device) * 8;
-    const unsigned grid = (unsigned)(want < most ? want : most);
+    const bool aligned = aligned_to(x, 16) && aligned_to(y, 16);
     with_dtype(dtype, [&](auto t) {
-        dropout_kernel<decltype(t)><<<grid, DROPOUT_THREADS, 0, s>>>(a);
+        using T = decltype(t);
+        constexpr int V = 16 / sizeof(T);
+        const long long per = (long long)(aligned ? V : 4) * DROPOUT_THREADS * DROPOUT_UNROLL;
+        const unsigned grid = (unsigned)((n + per - 1) / per);
+        if (aligned)
+            dropout_kernel<T, V, true><<<grid, DROPOUT_THREADS, 0, s>>>(a);
+        else
+            dropout_kernel<T, 4, false><<<grid, DROPOUT_THREADS, 0, s>>>(a);
         return 0;
     });
     count_launch();

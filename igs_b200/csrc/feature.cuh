@@ -34,6 +34,17 @@ inline auto with_dtype(int dtype, F&& f) {
     return f(float{});
 }
 
+// V neighbouring values as they lie in memory, moved by one load or store of up to 16 bytes
+// (aligned to its size).
+template <typename T, int V>
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
+    T v[V];
+};
+
+__host__ __device__ inline bool aligned_to(const void* p, size_t bytes) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
