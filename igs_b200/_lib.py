@@ -69,7 +69,7 @@ SIGNATURES = {
     "igs_embed_grad_workspace_bytes": (_i, [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)]),
     "igs_embed_grad": (_i, [_vp, _i, _i64, _vp, _i, _i64, _i64, _f, _i, _i64, _vp, _vp, _sz, _i, _vp]),
     "igs_layer_norm": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _f, _vp, _vp, _vp, _i, _vp]),
-    "igs_layer_norm_grad_workspace_bytes": (_sz, [_i64, _i64]),
+    "igs_layer_norm_grad_workspace_bytes": (_sz, [_i64, _i64, _i]),
     "igs_layer_norm_grad": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _vp, _i] + [_vp] * 6 + [_sz, _i, _vp]),
     "igs_dropout": (_i, [_vp, _i, _i64, ctypes.c_double, ctypes.c_ulonglong, ctypes.c_ulonglong, _vp, _vp, _i, _vp]),
     "igs_profile_enable": (_i, [_i]),
@@ -752,8 +752,8 @@ def layer_norm(x, weight, bias, wdtype, eps, stats):
 
 
 @functools.lru_cache(maxsize=256)
-def _layer_norm_grad_workspace_bytes(rows, D):
-    return int(load().igs_layer_norm_grad_workspace_bytes(rows, D))
+def _layer_norm_grad_workspace_bytes(rows, D, index):
+    return int(load().igs_layer_norm_grad_workspace_bytes(rows, D, index))
 
 
 def layer_norm_grad(dy, x, weight, wdtype, shift, rstd, want_x, want_weight, want_bias):
@@ -763,7 +763,7 @@ def layer_norm_grad(dy, x, weight, wdtype, shift, rstd, want_x, want_weight, wan
     dx = torch.empty((rows, D), dtype=x.dtype, device=dev) if want_x else None
     dw = torch.empty(D, dtype=wdtype, device=dev) if want_weight else None
     db = torch.empty(D, dtype=wdtype, device=dev) if want_bias else None
-    ws = _workspace(_layer_norm_grad_workspace_bytes(rows, D), dev)
+    ws = _workspace(_layer_norm_grad_workspace_bytes(rows, D, dev.index), dev)
     check("igs_layer_norm_grad",
           load().igs_layer_norm_grad(dy.data_ptr(), x.data_ptr(), FEATURE_DTYPES[x.dtype], rows, D,
                                      x.stride(0) if rows > 1 else D, weight.data_ptr() if weight is not None else None,

@@ -417,6 +417,7 @@ int igs_embed(const void* tokens, int token_bytes, long long n, const void* tabl
  * The table's gradient, by sorted tokens: d_table [rows,D] (contiguous, of dy's type) =
  * scale * the sum of dy's rows [n,D] (contiguous) over the places of each token, zero for rows
  * without one.  Every row is written.  Empty places and tokens outside the table add nothing.
+ * The workspace starts on a 16-byte boundary.
  * No floating-point atomics: the same bits on every call.
  */
 int igs_embed_grad_workspace_bytes(long long n, long long rows, long long D, int device, size_t* bytes);
@@ -441,7 +442,7 @@ int igs_layer_norm(const void* x, int dtype, long long rows, long long D, long l
  * when not wanted.  dy [rows,D] contiguous.  The column sums are taken over fixed blocks of
  * rows and added in a fixed order: the same bits on every call.
  */
-size_t igs_layer_norm_grad_workspace_bytes(long long rows, long long D);
+size_t igs_layer_norm_grad_workspace_bytes(long long rows, long long D, int device);
 int igs_layer_norm_grad(const void* dy, const void* x, int dtype, long long rows, long long D,
                         long long row_stride, const void* weight, int wdtype, const float* shift,
                         const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
