@@ -5,15 +5,16 @@
 // The gradient goes by sorted tokens instead of atomics: a stable sort of (token, place) puts the
 // places of one token next to each other in their own order, so every row is one sum in 32 bits
 // with a fixed sequence and one rounding, the same bits on every run.
-//   1. sort: least significant digits first, up to 10 bits a pass (a codebook of a million rows
-//      needs two); per pass a count per block of places, a prefix sum over blocks, and the
-//      placement.  Places without a token in the table drop out in the first pass.
+//   1. sort.  Up to RANK_MAX places: one kernel ranks every place against all keys.  More: least
+//      significant digits first, up to 10 bits a pass (a codebook of a million rows needs two); per
+//      pass a count per block of places, a prefix sum over blocks, and the placement.  Places
+//      without a token in the table drop out.
 //   2. segments: the sorted places are cut into chunks of equal length whatever the tokens are
 //      (one common token may own most of them).  A run of one token inside a chunk is finished
 //      there; the sums of runs that cross a border go to the chunk's two partial rows ("head":
 //      it came from the chunk before, "tail": it started here and goes on).  The same launch
 //      writes the zero rows.
-//   3. join: the chunk in which a crossing run started adds the run's partial rows in order.
+//   3. join: the partial rows of a crossing run are added in order.
 #include "feature.cuh"
 
 namespace igs {
@@ -59,21 +60,38 @@ struct EmbedArgs {
     float scale;
 };
 
-// one CTA per place (and on): a row of D values
-template <typename T>
-__global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(EmbedArgs a) {
-    for (long long i = blockIdx.x; i < a.n; i += gridDim.x) {
-        const long long tok = token_at(a.tokens, i);
-        const uint32_t row = row_of(a.tokens, tok);
-        T* out = static_cast<T*>(a.out) + i * a.D;
-        if (row != NO_ROW) {
-            const T* src = static_cast<const T*>(a.table) + (long long)row * a.row_stride;
-            for (long long c = threadIdx.x; c < a.D; c += EMBED_THREADS) out[c] = from_f<T>(to_f(src[c]) * a.scale);
-        } else {
+// A group of 2^log_g threads copies R rows, packs of V values a thread: the R tokens, then R
+// independent loads in flight per pack.
+template <typename T, int V, int R>
+__global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(EmbedArgs a, int log_g) {
+    const int lane = threadIdx.x & ((1 << log_g) - 1);
+    const long long i0 = ((long long)blockIdx.x * (EMBED_THREADS >> log_g) + (threadIdx.x >> log_g)) * R;
+    uint32_t row[R];
+    float none[R];  // what fills the row of a place without one
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        row[r] = NO_ROW;
+        none[r] = 0.f;
+        if (i0 + r < a.n) {
+            const long long tok = token_at(a.tokens, i0 + r);
+            row[r] = row_of(a.tokens, tok);
             // an empty place is zero; a token outside the table is an error that shows: NaN
-            const bool empty = a.tokens.has_empty && tok == a.tokens.empty;
-            const T v = from_f<T>(empty ? 0.f : __int_as_float(0x7fc00000));
-            for (long long c = threadIdx.x; c < a.D; c += EMBED_THREADS) out[c] = v;
+            if (!(a.tokens.has_empty && tok == a.tokens.empty)) none[r] = __int_as_float(0x7fc00000);
+        }
+    }
+    const long long packs = a.D / V;
+    for (long long p = lane; p < packs; p += 1 << log_g) {
+        Pack<T, V> v[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (row[r] != NO_ROW)
+                v[r] = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.table) + (long long)row[r] * a.row_stride)[p];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (i0 + r >= a.n) continue;
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[r].v[j] = from_f<T>(row[r] != NO_ROW ? to_f(v[r].v[j]) * a.scale : none[r]);
+            reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.out) + (i0 + r) * a.D)[p] = v[r];
         }
     }
 }
@@ -106,6 +124,64 @@ __device__ __forceinline__ bool sort_load(const SortArgs& a, long long i, long l
     key = row_of(a.tokens, token_at(a.tokens, i));
     place = (int)i;
     return key != NO_ROW;
+}
+
+// Few places: every place's slot is the number of keys below its own plus the number of equal ones
+// before it, counted over all keys.  Block b ranks the places 32 b .. 32 b + 31, one a lane; each
+// warp counts over a share of the keys.  n^2 comparisons, but one launch and no passes: 8192 places
+// are 67 million comparisons, a few microseconds over the whole device.
+constexpr int RANK_MAX = 8192;
+constexpr int RANK_WARPS = 16;
+__global__ void __launch_bounds__(RANK_WARPS * 32) sort_rank_kernel(SortArgs a) {
+    __shared__ __align__(16) uint32_t s_key[RANK_MAX];
+    __shared__ int s_rank[RANK_WARPS][32];
+    __shared__ int s_held[RANK_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int n = (int)a.n, padded = (n + 31) / 32 * 32;
+    int held = 0;
+    for (int i = threadIdx.x; i < padded; i += RANK_WARPS * 32) {
+        const uint32_t k = i < n ? row_of(a.tokens, token_at(a.tokens, i)) : NO_ROW;
+        s_key[i] = k;
+        held += k != NO_ROW;
+    }
+    __syncthreads();
+    const int mine = blockIdx.x * 32 + lane;
+    const uint32_t key = s_key[mine < padded ? mine : 0];
+    const int tiles = padded / 32, per = (tiles + RANK_WARPS - 1) / RANK_WARPS;
+    const int t1 = (warp + 1) * per < tiles ? (warp + 1) * per : tiles;
+    int rank = 0;
+    for (int t = warp * per; t < t1; ++t) {
+        const uint4* tile = reinterpret_cast<const uint4*>(s_key + t * 32);
+        if (t == blockIdx.x) {  // the block's own places: equal keys count when they come before
+            for (int j = 0; j < 32; ++j) rank += s_key[t * 32 + j] < key + (j < lane ? 1u : 0u);
+        } else {
+            const uint32_t below = key + (t < (int)blockIdx.x ? 1u : 0u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint4 k = tile[j];
+                rank += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
+            }
+        }
+    }
+    s_rank[warp][lane] = rank;
+    if (blockIdx.x == 0) {
+        held = __reduce_add_sync(0xffffffffu, held);
+        if (lane == 0) s_held[warp] = held;
+    }
+    __syncthreads();
+    if (warp) return;
+    int slot = 0;
+#pragma unroll
+    for (int w = 0; w < RANK_WARPS; ++w) slot += s_rank[w][lane];
+    if (mine < n && key != NO_ROW) {
+        a.keys_out[slot] = key;
+        a.places_out[slot] = mine;
+    }
+    if (blockIdx.x == 0 && lane == 0) {
+        int sum = 0;
+        for (int w = 0; w < RANK_WARPS; ++w) sum += s_held[w];
+        *a.count_out = sum;
+    }
 }
 
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(SortArgs a) {
@@ -234,11 +310,16 @@ struct SegmentArgs {
     long long rows, D;
     float scale;
     int chunks;
-    int sum_blocks, zero_blocks;
+    int sum_blocks;         // blocks of the segment kernel that sum; the others write zero rows
+    int log_g;              // a chunk is summed by 2^log_g threads, a pack of columns each
 };
 
-// positions [lo, hi) of a chunk
-__device__ __forceinline__ long long chunk_length(long long count, int chunks) { return (count + chunks - 1) / chunks; }
+constexpr int CHUNK_STEP = 8;  // places whose rows are loaded together; chunks are multiples of it
+
+// positions a chunk holds, the last one's less
+__device__ __forceinline__ long long chunk_length(long long count, int chunks) {
+    return ((count + chunks - 1) / chunks + CHUNK_STEP - 1) / CHUNK_STEP * CHUNK_STEP;
+}
 
 // whether a row has a token: binary search
 __device__ __forceinline__ bool has_key(const uint32_t* keys, int count, uint32_t row) {
@@ -250,74 +331,181 @@ __device__ __forceinline__ bool has_key(const uint32_t* keys, int count, uint32_
     return lo < count && keys[lo] == row;
 }
 
-// grid (sum blocks + zero blocks, column slabs).  Sum blocks: one chunk each, one column a thread.
-template <typename T>
+template <int V>
+__device__ __forceinline__ void store_part(float* part, const float (&sum)[V]) {
+    constexpr int Q = V < 4 ? V : 4;
+#pragma unroll
+    for (int j = 0; j < V; j += Q) {
+        Pack<float, Q> o;
+#pragma unroll
+        for (int i = 0; i < Q; ++i) o.v[i] = sum[j + i];
+        reinterpret_cast<Pack<float, Q>*>(part)[j / Q] = o;
+    }
+}
+
+// sum * scale to a row of the table
+template <typename T, int V>
+__device__ __forceinline__ void store_row(T* row, const float (&sum)[V], float scale) {
+    Pack<T, V> o;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.v[j] = from_f<T>(sum[j] * scale);
+    *reinterpret_cast<Pack<T, V>*>(row) = o;
+}
+
+// grid (sum blocks + zero blocks, column slabs).  Every thread owns one pack of V columns.
+template <typename T, int V>
 __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
     const int count = *a.count;
     T* d_table = static_cast<T*>(a.d_table);
-    const long long c = (long long)blockIdx.y * EMBED_THREADS + threadIdx.x;
+    const long long packs = a.D / V;
     if ((int)blockIdx.x >= a.sum_blocks) {
-        // rows without a token
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        const long long group = (long long)(blockIdx.x - a.sum_blocks) * (EMBED_THREADS / 32) + warp;
-        const long long groups = (long long)a.zero_blocks * (EMBED_THREADS / 32);
-        if (blockIdx.y) return;
-        for (long long r0 = group * 32; r0 < a.rows; r0 += groups * 32) {
+        // rows without a token: a warp looks up 32 rows at a time, then writes those that have none
+        const int lane = threadIdx.x & 31;
+        const long long first = (long long)blockIdx.y << a.log_g;
+        const long long last = first + (1ll << a.log_g) < packs ? first + (1ll << a.log_g) : packs;
+        const long long warps = (long long)(gridDim.x - a.sum_blocks) * (EMBED_THREADS / 32);
+        Pack<T, V> zero;
+#pragma unroll
+        for (int j = 0; j < V; ++j) zero.v[j] = from_f<T>(0.f);
+        for (long long r0 = ((long long)(blockIdx.x - a.sum_blocks) * (EMBED_THREADS / 32) + (threadIdx.x >> 5)) * 32;
+             r0 < a.rows; r0 += warps * 32) {
             const long long r = r0 + lane;
             unsigned absent = __ballot_sync(0xffffffffu, r < a.rows && !has_key(a.keys, count, (uint32_t)r));
             while (absent) {
                 const int k = __ffs(absent) - 1;
                 absent &= absent - 1;
-                for (long long i = lane; i < a.D; i += 32) d_table[(r0 + k) * a.D + i] = from_f<T>(0.f);
+                Pack<T, V>* row = reinterpret_cast<Pack<T, V>*>(d_table + (r0 + k) * a.D);
+                for (long long p = first + lane; p < last; p += 32) row[p] = zero;
             }
         }
         return;
     }
-    if (c >= a.D) return;
-    const long long len = chunk_length(count, a.chunks), lo = blockIdx.x * len;
+    const long long chunk = (long long)blockIdx.x * (EMBED_THREADS >> a.log_g) + (threadIdx.x >> a.log_g);
+    const long long pack = ((long long)blockIdx.y << a.log_g) + (threadIdx.x & ((1 << a.log_g) - 1));
+    const long long len = chunk_length(count, a.chunks), lo = chunk * len;
     const long long hi = lo + len < count ? lo + len : count;
-    if (lo >= hi) return;
-    const T* dy = static_cast<const T*>(a.dy);
+    if (chunk >= a.chunks || pack >= packs || lo >= hi) return;
+    const T* dy = static_cast<const T*>(a.dy) + pack * V;
+    d_table += pack * V;
+    float* part = a.part + chunk * 2 * a.D + pack * V;
     const bool from_before = lo > 0 && a.keys[lo - 1] == a.keys[lo];
     const bool goes_on = hi < count && a.keys[hi] == a.keys[hi - 1];
-    float* part = a.part + (long long)blockIdx.x * 2 * a.D;
     uint32_t key = a.keys[lo];
     bool first = true;
-    float sum = 0.f;
-    for (long long p = lo; p < hi; ++p) {
-        const uint32_t k = a.keys[p];
-        if (k != key) {
-            if (first && from_before)
-                part[c] = sum;
-            else
-                d_table[(long long)key * a.D + c] = from_f<T>(sum * a.scale);
-            first = false;
-            key = k;
-            sum = 0.f;
+    float sum[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = 0.f;
+    for (long long p = lo; p < hi; p += CHUNK_STEP) {
+        // (lo is a multiple of CHUNK_STEP and the sort's arrays are padded to 256 bytes: whole packs)
+        const Pack<uint32_t, 4>* kp = reinterpret_cast<const Pack<uint32_t, 4>*>(a.keys + p);
+        const Pack<int, 4>* pp = reinterpret_cast<const Pack<int, 4>*>(a.places + p);
+        Pack<uint32_t, 4> k[CHUNK_STEP / 4];
+        Pack<T, V> v[CHUNK_STEP];
+#pragma unroll
+        for (int q = 0; q < CHUNK_STEP / 4; ++q) {
+            k[q] = kp[q];
+            const Pack<int, 4> at = pp[q];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (p + q * 4 + i < hi) v[q * 4 + i] = *reinterpret_cast<const Pack<T, V>*>(dy + (long long)at.v[i] * a.D);
         }
-        sum += to_f(dy[(long long)a.places[p] * a.D + c]);
+#pragma unroll
+        for (int u = 0; u < CHUNK_STEP; ++u) {
+            if (p + u >= hi) break;
+            const uint32_t ku = k[u / 4].v[u % 4];
+            if (ku != key) {  // (the same in every thread of the group)
+                if (first && from_before) store_part(part, sum);
+                else store_row<T, V>(d_table + (long long)key * a.D, sum, a.scale);
+                first = false;
+                key = ku;
+#pragma unroll
+                for (int j = 0; j < V; ++j) sum[j] = 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] += to_f(v[u].v[j]);
+        }
     }
-    if (first && from_before)
-        part[c] = sum;
-    else if (goes_on)
-        part[a.D + c] = sum;
-    else
-        d_table[(long long)key * a.D + c] = from_f<T>(sum * a.scale);
+    if (first && from_before) store_part(part, sum);
+    else if (goes_on) store_part(part + a.D, sum);
+    else store_row<T, V>(d_table + (long long)key * a.D, sum, a.scale);
 }
 
-// grid (chunks, column slabs): the chunk in which a crossing run starts adds the run up
-template <typename T>
-__global__ void __launch_bounds__(EMBED_THREADS) join_kernel(SegmentArgs a) {
+// Runs that cross chunk borders: the tail of the chunk in which the run starts, then the heads of
+// the chunks that follow.  Q columns (4, or 1 where D is odd) a thread.
+//   Short runs, up to JOIN_SHORT heads: the first `chunks` blocks of a slab, one per chunk that may
+//   start one; a thread adds its columns up.
+//   Longer ones (they contain a chunk whose number is a multiple of JOIN_SHORT): one block per such
+//   chunk, which acts if it is the run's first.  32 threads across, 8 down: each of the 8 adds every
+//   8th row, and the 8 sums are added in order.
+constexpr int JOIN_SHORT = 16;
+constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_DOWN = JOIN_THREADS / 32;
+template <typename T, int Q>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(SegmentArgs a, int short_blocks, int short_slabs) {
+    __shared__ float s_sum[JOIN_DOWN][32 * Q];
     const int count = *a.count;
-    const long long len = chunk_length(count, a.chunks), lo = blockIdx.x * len, hi = lo + len;
-    const long long c = (long long)blockIdx.y * EMBED_THREADS + threadIdx.x;
-    if (c >= a.D || hi >= count) return;
-    const uint32_t key = a.keys[hi - 1];
-    if (a.keys[hi] != key) return;                                          // nothing crosses the border
-    if (lo > 0 && a.keys[lo] == key && a.keys[lo - 1] == key) return;       // it started further to the left
-    float sum = a.part[(long long)blockIdx.x * 2 * a.D + a.D + c];
-    for (long long k = blockIdx.x + 1; k * len < count && a.keys[k * len] == key; ++k) sum += a.part[k * 2 * a.D + c];
-    static_cast<T*>(a.d_table)[(long long)key * a.D + c] = from_f<T>(sum * a.scale);
+    const long long len = chunk_length(count, a.chunks);
+    // whether chunk k exists and begins with the key / in the middle of a run of it
+    const auto begins = [&](long long k, uint32_t key) { return k * len < count && a.keys[k * len] == key; };
+    const auto continues = [&](long long k, uint32_t key) { return k > 0 && begins(k, key) && a.keys[k * len - 1] == key; };
+    T* d_table = static_cast<T*>(a.d_table);
+    float sum[Q];
+
+    if ((int)blockIdx.x < short_blocks) {
+        const long long k0 = blockIdx.x / short_slabs;
+        const long long c = ((long long)(blockIdx.x % short_slabs) * JOIN_THREADS + threadIdx.x) * Q;
+        if ((k0 + 1) * len >= count) return;
+        const uint32_t key = a.keys[(k0 + 1) * len];
+        if (!continues(k0 + 1, key) || continues(k0, key)) return;  // nothing crosses, or it started before
+        if (begins(k0 + 1 + JOIN_SHORT, key) || c >= a.D) return;   // a long one
+        const Pack<float, Q> t = *reinterpret_cast<const Pack<float, Q>*>(a.part + (k0 * 2 + 1) * a.D + c);
+#pragma unroll
+        for (int j = 0; j < Q; ++j) sum[j] = t.v[j];
+        for (long long k = k0 + 1; begins(k, key); ++k) {
+            const Pack<float, Q> h = *reinterpret_cast<const Pack<float, Q>*>(a.part + k * 2 * a.D + c);
+#pragma unroll
+            for (int j = 0; j < Q; ++j) sum[j] += h.v[j];
+        }
+        store_row<T, Q>(d_table + (long long)key * a.D + c, sum, a.scale);
+        return;
+    }
+
+    const long long slabs = (a.D + 32 * Q - 1) / (32 * Q);
+    const long long b = blockIdx.x - short_blocks;
+    const long long m = (b / slabs + 1) * JOIN_SHORT;
+    const int across = threadIdx.x & 31, down = threadIdx.x >> 5;
+    const long long c = ((b % slabs) * 32 + across) * Q;
+    if (m * len >= count) return;
+    const uint32_t key = a.keys[m * len];
+    if (!continues(m, key)) return;
+    long long k0 = m - 1;  // back to the chunk in which the run starts
+    while (k0 > m - JOIN_SHORT && continues(k0, key)) --k0;
+    if (continues(k0, key)) return;  // the run holds an earlier multiple
+    if (!begins(k0 + 1 + JOIN_SHORT, key)) return;  // a short one
+    long long last = k0 + 1 + JOIN_SHORT, end = a.chunks;  // chunk `last` begins with the key, chunk `end` does not
+    while (end - last > 1) {
+        const long long mid = (last + end) / 2;
+        if (begins(mid, key)) last = mid; else end = mid;
+    }
+#pragma unroll
+    for (int j = 0; j < Q; ++j) sum[j] = 0.f;
+    if (c < a.D) {
+#pragma unroll 4
+        for (long long k = k0 + down; k <= last; k += JOIN_DOWN) {
+            const Pack<float, Q> h = *reinterpret_cast<const Pack<float, Q>*>(a.part + (k * 2 + (k == k0)) * a.D + c);
+#pragma unroll
+            for (int j = 0; j < Q; ++j) sum[j] += h.v[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < Q; ++j) s_sum[down][across * Q + j] = sum[j];
+    __syncthreads();
+    if (down || c >= a.D) return;
+    for (int d = 1; d < JOIN_DOWN; ++d) {
+#pragma unroll
+        for (int j = 0; j < Q; ++j) sum[j] += s_sum[d][across * Q + j];
+    }
+    store_row<T, Q>(d_table + (long long)key * a.D + c, sum, a.scale);
 }
 
 // ---------------------------------------------------------------------------
@@ -335,10 +523,12 @@ static int plan_embed_grad(long long n, long long rows, long long D, int device,
     p->passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
     p->bits = (bits + p->passes - 1) / p->passes;
     p->n_blocks = (int)((n + SORT_BLOCK - 1) / SORT_BLOCK);
-    // enough chunks to fill the device once the column slabs are counted, none shorter than 16 places
-    const long long slabs = (D + EMBED_THREADS - 1) / EMBED_THREADS;
-    long long chunks = (long long)sm_count(device) * 16 / slabs;
-    if (chunks > (n + 15) / 16) chunks = (n + 15) / 16;
+    // enough chunks to fill the device with threads of one 16-byte pack each, none shorter than
+    // CHUNK_STEP places (packs of 4 values are counted: half as many threads do for 16-bit ones)
+    const long long threads_per_chunk = (D + 3) / 4;
+    long long chunks = (long long)sm_count(device) * 1024 / threads_per_chunk;
+    if (chunks < sm_count(device) / 4) chunks = sm_count(device) / 4;
+    if (chunks > (n + CHUNK_STEP - 1) / CHUNK_STEP) chunks = (n + CHUNK_STEP - 1) / CHUNK_STEP;
     p->chunks = (int)(chunks < 1 ? 1 : chunks);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -356,6 +546,15 @@ static int plan_embed_grad(long long n, long long rows, long long D, int device,
     p->off_part = take((size_t)p->chunks * 2 * D * 4);
     p->bytes = at;
     return IGS_OK;
+}
+
+// log2 of the threads that share a row of `packs` packs: the narrowest power of two that covers
+// it, a whole block at most
+static int group_log(long long packs) {
+    int g = 0;
+    while (g < 7 && (1 << g) < packs) ++g;
+    static_assert(EMBED_THREADS == 1 << 7, "a block is the widest group");
+    return g;
 }
 
 static int token_args_ok(int token_bytes, long long n, long long rows, long long D, int dtype, float scale) {
@@ -381,8 +580,23 @@ extern "C" int igs_embed(const void* tokens, int token_bytes, long long n, const
     if (!guard.ok) return IGS_ERR_DEVICE;
     cudaStream_t s = (cudaStream_t)stream;
     EmbedArgs a{{tokens, token_bytes == 8, has_empty != 0, empty, rows}, table, out, n, D, row_stride, scale};
+    const size_t size = dtype_size(dtype);
+    const bool packed = aligned_to(table, 16) && aligned_to(out, 16) && (size_t)D * size % 16 == 0 &&
+                        (size_t)row_stride * size % 16 == 0;
+    const long long packs = packed ? D * (long long)size / 16 : D;
+    const int log_g = group_log(packs);
+    // four rows a group once that still leaves every SM sixteen blocks; below, latency counts
+    const long long groups = EMBED_THREADS >> log_g;
+    const bool four = n >= (long long)sm_count(device) * 16 * groups * 4;
+    const long long per = groups * (four ? 4 : 1);
+    const unsigned grid = (unsigned)((n + per - 1) / per);
     with_dtype(dtype, [&](auto t) {
-        embed_kernel<decltype(t)><<<(unsigned)n, EMBED_THREADS, 0, s>>>(a);
+        using T = decltype(t);
+        constexpr int V = 16 / sizeof(T);
+        if (packed && four) embed_kernel<T, V, 4><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
+        else if (packed) embed_kernel<T, V, 1><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
+        else if (four) embed_kernel<T, 1, 4><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
+        else embed_kernel<T, 1, 1><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
         return 0;
     });
     count_launch();
@@ -407,7 +621,7 @@ extern "C" int igs_embed_grad(const void* tokens, int token_bytes, long long n, 
     EmbedPlan p;
     rc = plan_embed_grad(n, rows, D, device, &p);
     if (rc) return rc;
-    if (n > 0 && (!workspace || workspace_bytes < p.bytes)) return IGS_ERR_WORKSPACE;
+    if (n > 0 && (!workspace || workspace_bytes < p.bytes || !aligned_to(workspace, 16))) return IGS_ERR_WORKSPACE;
     DeviceGuard guard(device);
     if (!guard.ok) return IGS_ERR_DEVICE;
     cudaStream_t s = (cudaStream_t)stream;
@@ -423,7 +637,15 @@ extern "C" int igs_embed_grad(const void* tokens, int token_bytes, long long n, 
     so.n = n;
     so.n_blocks = p.n_blocks;
     so.digits = 1 << p.bits;
-    for (int pass = 0; pass < p.passes; ++pass) {
+    const int passes = n <= RANK_MAX ? 0 : p.passes;
+    if (!passes) {
+        so.keys_out = reinterpret_cast<uint32_t*>(ws + p.off_keys[0]);
+        so.places_out = reinterpret_cast<int*>(ws + p.off_places[0]);
+        so.count_out = count;
+        sort_rank_kernel<<<(unsigned)((n + 31) / 32), RANK_WARPS * 32, 0, s>>>(so);
+        count_launch();
+    }
+    for (int pass = 0; pass < passes; ++pass) {
         const int to = pass & 1;
         so.keys_in = pass ? reinterpret_cast<uint32_t*>(ws + p.off_keys[to ^ 1]) : nullptr;
         so.places_in = pass ? reinterpret_cast<int*>(ws + p.off_places[to ^ 1]) : nullptr;
@@ -436,17 +658,28 @@ extern "C" int igs_embed_grad(const void* tokens, int token_bytes, long long n, 
         sort_place_kernel<<<p.n_blocks, SORT_THREADS, 0, s>>>(so);
         count_launch(3);
     }
+    const bool packed = aligned_to(dy, 16) && aligned_to(d_table, 16) && (size_t)D * dtype_size(dtype) % 16 == 0;
+    const long long packs = packed ? D * (long long)dtype_size(dtype) / 16 : D;
+    const int log_g = group_log(packs), groups = EMBED_THREADS >> log_g;
     SegmentArgs a{so.keys_out, so.places_out, count, dy, d_table, reinterpret_cast<float*>(ws + p.off_part), rows, D,
-                  scale, p.chunks, p.chunks, 0};
+                  scale, p.chunks, (p.chunks + groups - 1) / groups, log_g};
     const long long zero = (rows + EMBED_THREADS - 1) / EMBED_THREADS;
-    a.zero_blocks = (int)(zero < 4096 ? zero : 4096);
-    const unsigned slabs = (unsigned)((D + EMBED_THREADS - 1) / EMBED_THREADS);
+    const dim3 grid((unsigned)(a.sum_blocks + (zero < 4096 ? zero : 4096)), (unsigned)((packs + (1 << log_g) - 1) >> log_g));
+    const long long q = packed ? 4 : 1;
+    const long long short_slabs = (D + JOIN_THREADS * q - 1) / (JOIN_THREADS * q), long_slabs = (D + 32 * q - 1) / (32 * q);
+    const long long short_blocks = (p.chunks - 1) * short_slabs, long_blocks = (p.chunks - 1) / JOIN_SHORT * long_slabs;
+    const unsigned joins = (unsigned)(short_blocks + long_blocks);
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        segment_kernel<T><<<dim3((unsigned)(a.sum_blocks + a.zero_blocks), slabs), EMBED_THREADS, 0, s>>>(a);
-        if (a.chunks > 1) join_kernel<T><<<dim3((unsigned)a.chunks, slabs), EMBED_THREADS, 0, s>>>(a);
+        if (packed) {
+            segment_kernel<T, 16 / sizeof(T)><<<grid, EMBED_THREADS, 0, s>>>(a);
+            if (joins) join_kernel<T, 4><<<joins, JOIN_THREADS, 0, s>>>(a, (int)short_blocks, (int)short_slabs);
+        } else {
+            segment_kernel<T, 1><<<grid, EMBED_THREADS, 0, s>>>(a);
+            if (joins) join_kernel<T, 1><<<joins, JOIN_THREADS, 0, s>>>(a, (int)short_blocks, (int)short_slabs);
+        }
         return 0;
     });
-    count_launch(a.chunks > 1 ? 2 : 1);
+    count_launch(joins ? 2 : 1);
     return (int)cudaGetLastError();
 }
