@@ -117,6 +117,29 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_features = None
+
+
+def features():
+    """The torch binding of the feature operators (``_features.so``), built first when it is missing
+    or out of date, like the library it calls."""
+    global _features
+    if _features is None:
+        load()
+        with _lock:
+            if _features is None:
+                from . import build as _build
+
+                try:
+                    _build.build_binding()
+                    from . import _features as ext
+                except Exception as exc:  # noqa: BLE001 - surfaced verbatim below
+                    raise ImportError(f"igs_b200: {_build.BINDING_PATH} is missing or out of date and could not be built "
+                                      f"({exc}). Run `python -m igs_b200.build`; there is no fallback.") from exc
+                _features = ext
+    return _features
+
+
 def check(fn: str, code: int) -> None:
     if code != 0:
         raise IgsError(fn, code, load().igs_strerror(code).decode())
@@ -694,94 +717,6 @@ def mse_grad(out: torch.Tensor, target: torch.Tensor, upstream: torch.Tensor | N
     check("igs_mse_grad", load().igs_mse_grad(_ptr(out), _ptr(target), out.numel(), _ptr(upstream), _ptr(gout),
                                               dev.index, _stream(dev)))
     return gout
-
-
-# element types of the feature operators (include/igs_b200.h)
-FEATURE_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def embed(tokens, table, scale, empty):
-    """out [n,D] = scale * table[tokens]; tokens [n] contiguous int32 / int64, table [rows,D] with
-    inner stride 1; empty: the token of a place without one, or None."""
-    dev = table.device
-    n = tokens.numel()
-    rows, D = table.shape
-    out = torch.empty((n, D), dtype=table.dtype, device=dev)
-    check("igs_embed",
-          load().igs_embed(tokens.data_ptr(), tokens.element_size(), n, table.data_ptr(), FEATURE_DTYPES[table.dtype],
-                           rows, D, table.stride(0) if rows > 1 else D, scale, empty is not None, empty or 0,
-                           out.data_ptr(), dev.index, _stream(dev)))
-    return out
-
-
-@functools.lru_cache(maxsize=256)
-def _embed_grad_workspace_bytes(n, rows, D, index):
-    b = _sz(0)
-    check("igs_embed_grad_workspace_bytes",
-          load().igs_embed_grad_workspace_bytes(n, rows, D, index, ctypes.byref(b)))
-    return int(b.value)
-
-
-def embed_grad(tokens, dy, rows, scale, empty):
-    """d_table [rows,D] from dy [n,D] (contiguous): scale * the sums over the places of each token."""
-    dev = dy.device
-    n, D = dy.shape
-    d_table = torch.empty((rows, D), dtype=dy.dtype, device=dev)
-    ws = _workspace(_embed_grad_workspace_bytes(n, rows, D, dev.index), dev)
-    check("igs_embed_grad",
-          load().igs_embed_grad(tokens.data_ptr(), tokens.element_size(), n, dy.data_ptr(), FEATURE_DTYPES[dy.dtype],
-                                rows, D, scale, empty is not None, empty or 0, d_table.data_ptr(), ws.data_ptr(),
-                                ws.numel(), dev.index, _stream(dev)))
-    return d_table
-
-
-def layer_norm(x, weight, bias, wdtype, eps, stats):
-    """x [rows,D] with inner stride 1 -> (y, shift, rstd); shift and rstd None without stats."""
-    dev = x.device
-    rows, D = x.shape
-    y = torch.empty((rows, D), dtype=x.dtype, device=dev)
-    shift = torch.empty(rows, dtype=torch.float32, device=dev) if stats else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if stats else None
-    check("igs_layer_norm",
-          load().igs_layer_norm(x.data_ptr(), FEATURE_DTYPES[x.dtype], rows, D, x.stride(0) if rows > 1 else D,
-                                weight.data_ptr() if weight is not None else None,
-                                bias.data_ptr() if bias is not None else None, FEATURE_DTYPES[wdtype], eps, y.data_ptr(),
-                                shift.data_ptr() if stats else None, rstd.data_ptr() if stats else None, dev.index,
-                                _stream(dev)))
-    return y, shift, rstd
-
-
-@functools.lru_cache(maxsize=256)
-def _layer_norm_grad_workspace_bytes(rows, D, index):
-    return int(load().igs_layer_norm_grad_workspace_bytes(rows, D, index))
-
-
-def layer_norm_grad(dy, x, weight, wdtype, shift, rstd, want_x, want_weight, want_bias):
-    """-> (dx, dweight, dbias), None for those not wanted; dy [rows,D] contiguous."""
-    dev = x.device
-    rows, D = x.shape
-    dx = torch.empty((rows, D), dtype=x.dtype, device=dev) if want_x else None
-    dw = torch.empty(D, dtype=wdtype, device=dev) if want_weight else None
-    db = torch.empty(D, dtype=wdtype, device=dev) if want_bias else None
-    ws = _workspace(_layer_norm_grad_workspace_bytes(rows, D, dev.index), dev)
-    check("igs_layer_norm_grad",
-          load().igs_layer_norm_grad(dy.data_ptr(), x.data_ptr(), FEATURE_DTYPES[x.dtype], rows, D,
-                                     x.stride(0) if rows > 1 else D, weight.data_ptr() if weight is not None else None,
-                                     FEATURE_DTYPES[wdtype], shift.data_ptr(), rstd.data_ptr(),
-                                     dx.data_ptr() if want_x else None, dw.data_ptr() if want_weight else None,
-                                     db.data_ptr() if want_bias else None, ws.data_ptr(), ws.numel(), dev.index,
-                                     _stream(dev)))
-    return dx, dw, db
-
-
-def dropout(x, p, seed, offset, state):
-    """x contiguous; seed and offset 64-bit numbers; state: None or two int64 on x's device."""
-    dev = x.device
-    y = torch.empty_like(x)
-    check("igs_dropout",
-          load().igs_dropout(x.data_ptr(), FEATURE_DTYPES[x.dtype], x.numel(), p, seed, offset,
-                             state.data_ptr() if state is not None else None, y.data_ptr(), dev.index, _stream(dev)))
-    return y
 
 
 KERNEL_NAMES = ("pack", "forward", "reduce_normalize", "pixel_terms", "backward", "finalize", "coord_grad", "grid_check")

@@ -1,10 +1,12 @@
-"""Builds ``libigs_b200.so`` (the CUDA kernels + C ABI) in-tree with nvcc for sm_100a.
+"""Builds ``libigs_b200.so`` (the CUDA kernels + C ABI) in-tree with nvcc for sm_100a, and
+``_features.so`` (the torch binding of the feature operators) with g++.
 
     python -m igs_b200.build            # build if stale
     python -m igs_b200.build --force
 
-The shared object sits beside this file so that it travels with the source tree; it
-links only against the CUDA runtime (no torch, no Python).
+The shared objects sit beside this file so that they travel with the source tree.  The
+library links only against the CUDA runtime (no torch, no Python); the binding holds no
+kernels and links against the library and torch.
 """
 from __future__ import annotations
 
@@ -101,5 +103,66 @@ def _build_locked(verbose: bool) -> str:
     return LIB_PATH
 
 
+# ---------------------------------------------------------------------------
+# the torch binding of the feature operators
+# ---------------------------------------------------------------------------
+BINDING_SRC = os.path.join(CSRC, "binding", "features.cpp")
+BINDING_PATH = os.path.join(HERE, "_features.so")
+BINDING_STAMP = BINDING_PATH + ".srchash"
+BINDING_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wl,-rpath,$ORIGIN"]
+
+
+def binding_hash() -> str:
+    """Hash of the binding's source, the library's header, the flags, and the torch and Python
+    it was compiled against."""
+    import torch
+
+    h = hashlib.sha256(" ".join([*BINDING_FLAGS, torch.__version__, sys.version]).encode())
+    for path in (BINDING_SRC, os.path.join(INCLUDE, "igs_b200.h")):
+        with open(path, "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()
+
+
+def binding_is_stale() -> bool:
+    if not os.path.exists(BINDING_PATH) or not os.path.exists(BINDING_STAMP):
+        return True
+    with open(BINDING_STAMP) as f:
+        return f.read().strip() != binding_hash()
+
+
+def build_binding(force: bool = False) -> str:
+    """Builds the binding if it is stale (the library, which it links against, first)."""
+    build()
+    if not force and not binding_is_stale():
+        return BINDING_PATH
+    with open(BINDING_PATH + ".lock", "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        if not force and not binding_is_stale():
+            return BINDING_PATH
+        import sysconfig
+
+        import torch
+
+        digest = binding_hash()
+        base = os.path.dirname(torch.__file__)
+        libs = os.path.join(base, "lib")
+        cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+        includes = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+                    os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+        cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
+        cmd = [cxx, *BINDING_FLAGS, *[f for i in includes for f in ("-isystem", i)],
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", BINDING_SRC, "-o", BINDING_PATH,
+               "-L", HERE, "-l:libigs_b200.so", "-L", libs, f"-Wl,-rpath,{libs}", "-ltorch_python", "-ltorch",
+               "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("g++ failed:\n" + (res.stdout + res.stderr)[-4000:])
+        with open(BINDING_STAMP, "w") as f:
+            f.write(digest + "\n")
+        return BINDING_PATH
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
+    print(build_binding(force="--force" in sys.argv))
