@@ -68,9 +68,9 @@ SIGNATURES = {
     "igs_embed": (_i, [_vp, _i, _i64, _vp, _i, _i64, _i64, _i64, _f, _i, _i64, _vp, _i, _vp]),
     "igs_embed_grad_workspace_bytes": (_i, [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)]),
     "igs_embed_grad": (_i, [_vp, _i, _i64, _vp, _i, _i64, _i64, _f, _i, _i64, _vp, _vp, _sz, _i, _vp]),
-    "igs_layer_norm": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _f, _vp, _vp, _vp, _i, _vp]),
+    "igs_layer_norm": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _f, _vp, _vp, _i, _vp]),
     "igs_layer_norm_grad_workspace_bytes": (_sz, [_i64, _i64, _i]),
-    "igs_layer_norm_grad": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _vp, _i] + [_vp] * 6 + [_sz, _i, _vp]),
+    "igs_layer_norm_grad": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _vp, _i] + [_vp] * 5 + [_sz, _i, _vp]),
     "igs_dropout": (_i, [_vp, _i, _i64, ctypes.c_double, ctypes.c_ulonglong, ctypes.c_ulonglong, _vp, _vp, _i, _vp]),
     "igs_profile_enable": (_i, [_i]),
     "igs_profile_reset": (_i, []),

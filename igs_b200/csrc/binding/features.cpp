@@ -191,7 +191,7 @@ bool as_rows(const Tensor& x, Rows& r) {
 
 struct NormBackward : torch::autograd::Node {
     SavedVariable x_, weight_;
-    Tensor stats;  // [2, rows]: shift, rstd
+    Tensor stats;  // [rows, 4]
     Rows rows;
     at::ScalarType wtype;
 
@@ -209,10 +209,9 @@ struct NormBackward : torch::autograd::Node {
             bytes = igs_layer_norm_grad_workspace_bytes(rows.count, rows.width, device_index(dy));
             ws = workspace(bytes, dy);
         }
-        const float* shift = stats.data_ptr<float>();
         check("igs_layer_norm_grad",
               igs_layer_norm_grad(dy.data_ptr(), x.data_ptr(), type_code(dy.scalar_type()), rows.count, rows.width,
-                                  rows.stride, data(weight), type_code(wtype), shift, shift + rows.count, data(res[0]),
+                                  rows.stride, data(weight), type_code(wtype), stats.data_ptr<float>(), data(res[0]),
                                   data(res[1]), data(res[2]), data(ws), bytes, device_index(dy), stream_of(dy)));
         return once(std::move(res));
     }
@@ -263,11 +262,10 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const s
         const Tensor b = given[1].defined() ? given[1].contiguous() : Tensor();
         y = at::empty(x.sizes(), x.options());
         Tensor stats;
-        if (grad) stats = at::empty({2, r.count}, x.options().dtype(at::kFloat));
-        float* shift = grad ? stats.data_ptr<float>() : nullptr;
+        if (grad) stats = at::empty({r.count, 4}, x.options().dtype(at::kFloat));
         check("igs_layer_norm",
               igs_layer_norm(src.data_ptr(), type_code(x.scalar_type()), r.count, D, r.stride, data(w), data(b),
-                             type_code(wtype), e, y.data_ptr(), shift, grad ? shift + r.count : nullptr, device_index(x),
+                             type_code(wtype), e, y.data_ptr(), grad ? stats.data_ptr<float>() : nullptr, device_index(x),
                              stream_of(x)));
         if (grad) {
             node = make_node<NormBackward>();

@@ -41,6 +41,124 @@ struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
     T v[V];
 };
 
+// V values in 32 bits.  Pairs of neighbours share a packed f32x2 operand: half the instructions to
+// issue for the same arithmetic.
+template <int V>
+struct Vals {
+    static_assert(V % 2 == 0, "pairs");
+    f2 v[V / 2];
+};
+template <>
+struct Vals<1> {
+    float v;
+};
+
+template <int V>
+__device__ __forceinline__ Vals<V> splat(float x) {
+    Vals<V> r;
+    if constexpr (V == 1) r.v = x;
+    else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) r.v[i] = pk(x, x);
+    }
+    return r;
+}
+
+__device__ __forceinline__ f2 pair_f(const float* p) { return pk(p[0], p[1]); }
+__device__ __forceinline__ f2 pair_f(const __nv_bfloat16* p) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);  // a bfloat16 is the upper half of a float
+    return pk(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ f2 pair_f(const __half* p) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(p));
+    return pk(f.x, f.y);
+}
+template <typename T, int V>
+__device__ __forceinline__ Vals<V> to_vals(const Pack<T, V>& p) {
+    Vals<V> r;
+    if constexpr (V == 1) r.v = to_f(p.v[0]);
+    else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) r.v[i] = pair_f(p.v + 2 * i);
+    }
+    return r;
+}
+
+__device__ __forceinline__ void put_pair(float* p, float a, float b) {
+    p[0] = a;
+    p[1] = b;
+}
+__device__ __forceinline__ void put_pair(__nv_bfloat16* p, float a, float b) {
+    *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b);
+}
+__device__ __forceinline__ void put_pair(__half* p, float a, float b) {
+    *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b);
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> to_pack(const Vals<V>& x) {
+    Pack<T, V> r;
+    if constexpr (V == 1) r.v[0] = from_f<T>(x.v);
+    else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            float a, b;
+            upk(x.v[i], a, b);
+            put_pair(r.v + 2 * i, a, b);
+        }
+    }
+    return r;
+}
+
+template <int V>
+__device__ __forceinline__ Vals<V> add(Vals<V> a, const Vals<V>& b) {
+    if constexpr (V == 1) a.v += b.v;
+    else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) a.v[i] = add2(a.v[i], b.v[i]);
+    }
+    return a;
+}
+template <int V>
+__device__ __forceinline__ Vals<V> sub(Vals<V> a, const Vals<V>& b) {
+    if constexpr (V == 1) a.v -= b.v;
+    else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) a.v[i] = sub2(a.v[i], b.v[i]);
+    }
+    return a;
+}
+template <int V>
+__device__ __forceinline__ Vals<V> mul(Vals<V> a, const Vals<V>& b) {
+    if constexpr (V == 1) a.v *= b.v;
+    else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) a.v[i] = mul2(a.v[i], b.v[i]);
+    }
+    return a;
+}
+// a b + c
+template <int V>
+__device__ __forceinline__ Vals<V> fma(const Vals<V>& a, const Vals<V>& b, Vals<V> c) {
+    if constexpr (V == 1) c.v = fmaf(a.v, b.v, c.v);
+    else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) c.v[i] = fma2(a.v[i], b.v[i], c.v[i]);
+    }
+    return c;
+}
+template <int V>
+__device__ __forceinline__ float total(const Vals<V>& a) {
+    if constexpr (V == 1) return a.v;
+    else {
+        f2 t = a.v[0];
+#pragma unroll
+        for (int i = 1; i < V / 2; ++i) t = add2(t, a.v[i]);
+        float lo, hi;
+        upk(t, lo, hi);
+        return lo + hi;
+    }
+}
+
 __host__ __device__ inline bool aligned_to(const void* p, size_t bytes) {
     return reinterpret_cast<uintptr_t>(p) % bytes == 0;
 }

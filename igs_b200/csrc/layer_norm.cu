@@ -21,15 +21,13 @@ struct NormArgs {
     const void* w;  // NULL: ones
     const void* b;  // NULL: zeros
     void* y;
-    float* shift;   // NULL, or [rows]
-    float* rstd;    // NULL, or [rows]
+    RowStats* stats;  // NULL, or [rows]
     long long rows, D, row_stride;
     float eps;
 };
 
-// Rows that fit the registers of a group of G threads, ITEMS packs of V values a thread: one read
-// of x, one write of y.  A group takes R rows at a time, so that their sums overlap and a weight
-// is loaded once for all of them.
+// Few rows, where latency counts: a group of G threads holds R rows in registers, ITEMS packs of V
+// values a thread, and every row has its own group.
 template <typename T, typename W, int V, int G, int ITEMS, int R>
 __global__ void __launch_bounds__(norm_block(G)) layer_norm_kernel(NormArgs a) {
     constexpr int GROUPS = norm_block(G) / G;
@@ -39,13 +37,14 @@ __global__ void __launch_bounds__(norm_block(G)) layer_norm_kernel(NormArgs a) {
     const int packs = (int)(a.D / V);
     const long long row0 = ((long long)blockIdx.x * GROUPS + threadIdx.x / G) * R;
     // (a group past the last row stays to take part in its warp's or block's sums)
+    const int left = (int)(a.rows - row0 < R ? a.rows - row0 : R);
 
     Pack<T, V> x[R][ITEMS];
-    float x0[R], sum[R], rstd[R];
+    float x0[R], shift[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const T* src = static_cast<const T*>(a.x) + (row0 + r) * a.row_stride;
-        const bool ok = row0 + r < a.rows;
+        const bool ok = r < left;
         x0[r] = ok ? to_f(src[0]) : 0.f;
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {
@@ -55,55 +54,179 @@ __global__ void __launch_bounds__(norm_block(G)) layer_norm_kernel(NormArgs a) {
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        sum[r] = 0.f;
+        Vals<V> sum = splat<V>(0.f);
+        const Vals<V> first = splat<V>(x0[r]);
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k)
-            if (k * G + lane < packs && row0 + r < a.rows) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) sum[r] += to_f(x[r][k].v[j]) - x0[r];
-            }
+            if (k * G + lane < packs && r < left) sum = add(sum, sub(to_vals<T, V>(x[r][k]), first));
+        shift[r] = total(sum);
     }
-    group_sum<G, R>(sum, s_red, 0);
+    group_sum<G, R>(shift, s_red, 0);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        sum[r] *= inv_d;  // the shift
-        rstd[r] = 0.f;
+        shift[r] *= inv_d;
+        Vals<V> sq = splat<V>(0.f);
+        const Vals<V> first = splat<V>(x0[r]), mean = splat<V>(shift[r]);
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k)
-            if (k * G + lane < packs && row0 + r < a.rows) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float d = (to_f(x[r][k].v[j]) - x0[r]) - sum[r];
-                    rstd[r] = fmaf(d, d, rstd[r]);
-                }
+            if (k * G + lane < packs && r < left) {
+                const Vals<V> d = sub(sub(to_vals<T, V>(x[r][k]), first), mean);
+                sq = fma(d, d, sq);
             }
+        rstd[r] = total(sq);
     }
     group_sum<G, R>(rstd, s_red, 1);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        rstd[r] = 1.f / sqrtf(rstd[r] * inv_d + a.eps);
-        if (lane == 0 && a.shift && row0 + r < a.rows) {
-            a.shift[row0 + r] = sum[r];
-            a.rstd[row0 + r] = rstd[r];
-        }
+        rstd[r] = rsqrtf(rstd[r] * inv_d + a.eps);
+        if (lane == 0 && a.stats && r < left) a.stats[row0 + r] = RowStats{x0[r], shift[r], rstd[r], 0.f};
     }
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         const int p = k * G + lane;
         if (p >= packs) continue;
-        float w[V], b[V];
-        load_weights<W, V>(a.w, (long long)p * V, 1.f, w);
-        load_weights<W, V>(a.b, (long long)p * V, 0.f, b);
+        const Vals<V> w = load_weights<W, V>(a.w, p, 1.f), b = load_weights<W, V>(a.b, p, 0.f);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (row0 + r >= a.rows) continue;
-            Pack<T, V> y;
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                y.v[j] = from_f<T>(fmaf(((to_f(x[r][k].v[j]) - x0[r]) - sum[r]) * rstd[r], w[j], b[j]));
-            reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + (row0 + r) * a.D)[p] = y;
+            if (r >= left) continue;
+            const Vals<V> d = sub(sub(to_vals<T, V>(x[r][k]), splat<V>(x0[r])), splat<V>(shift[r]));
+            const Vals<V> y = fma(mul(d, splat<V>(rstd[r])), w, b);
+            reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + (row0 + r) * a.D)[p] = to_pack<T, V>(y);
         }
     }
+}
+
+// Many rows: blocks stay and rows stream by, R at a time a group, so that the weights are read from
+// memory once a block, and each thread copies its packs of the next batches to shared memory of its own
+// ahead of time (cp.async), so that memory does not wait for a row's two sums.
+template <typename T, typename W, int V, int G, int ITEMS, int FULL, int R>
+__global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stream_kernel(NormArgs a) {
+    constexpr int BLOCK = norm_block(G), GROUPS = BLOCK / G, PACK = sizeof(Pack<T, V>);
+    constexpr bool ASYNC = norm_async<T, V>;
+    constexpr int STAGES = norm_stages<T, V>(ITEMS * R, BLOCK);
+    extern __shared__ __align__(16) unsigned char s_mem[];
+    __shared__ float s_red[G > 32 ? 2 * (G / 32) * R : 1];
+    const int lane = threadIdx.x % G, group = threadIdx.x / G;
+    const float inv_d = 1.f / (float)a.D;
+    const int packs = (int)(a.D / V), mine = packs - lane;  // (item k is there when k G < mine)
+    const long long step = (long long)gridDim.x * (GROUPS * R);
+
+    // shared memory: the ring, slot [stage][row][item][thread]; then weights and biases
+    Pack<T, V>* ring = reinterpret_cast<Pack<T, V>*>(s_mem) + threadIdx.x;
+    const auto slot = [&](int stage, int r, int k) { return ring + ((stage * R + r) * ITEMS + k) * BLOCK; };
+    float* s_w = reinterpret_cast<float*>(s_mem + (ASYNC ? STAGES * R * ITEMS * BLOCK * PACK : 0));
+    float* s_b = s_w + a.D;
+
+    // (addresses advance by a fixed number of bytes: this thread's first pack of a batch's first row)
+    const long long first = (long long)blockIdx.x * (GROUPS * R) + group * R;
+    const long long x_row = a.row_stride * (long long)sizeof(T), y_row = a.D * (long long)sizeof(T);
+    const char* ahead = static_cast<const char*>(a.x) + first * x_row + lane * PACK;
+    const char* firsts = static_cast<const char*>(a.x) + first * x_row;
+    char* out = static_cast<char*>(a.y) + first * y_row + lane * PACK;
+    const char* now = ahead;  // (used where nothing is copied ahead)
+    long long ahead_left = a.rows - first;
+    const auto fetch = [&](int stage) {
+        const int n = (int)(ahead_left < R ? ahead_left : R);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (r >= n) break;
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k)
+                if (k < FULL || k * G < mine) copy_async<PACK>(slot(stage, r, k), ahead + r * x_row + k * (G * PACK));
+        }
+        ahead += step * x_row;
+        ahead_left -= step;
+    };
+    if constexpr (ASYNC) {
+#pragma unroll
+        for (int q = 0; q < STAGES - 1; ++q) {
+            fetch(q);
+            copy_commit();
+        }
+    }
+    stage_weights<W, V>(s_w, a.w, 1.f, (int)a.D, packs, BLOCK);
+    stage_weights<W, V>(s_b, a.b, 0.f, (int)a.D, packs, BLOCK);
+    // A row's first value: lane 0 holds it; in groups wider than a warp it is loaded one batch ahead.
+    float next[R];
+    const auto fetch_first = [&](long long rows_left) {
+        if constexpr (G > 32) {
+            const int n = (int)(rows_left < R ? rows_left : R);
+#pragma unroll
+            for (int r = 0; r < R; ++r) next[r] = r < n ? to_f(*reinterpret_cast<const T*>(firsts + r * x_row)) : 0.f;
+            firsts += step * x_row;
+        }
+    };
+    fetch_first(a.rows - first);
+    __syncthreads();
+
+    int stage = 0;
+    // (a warp goes on while it has a row; narrower groups share one and go on together, a wider group
+    // is the block: barriers and exchanges are met by all of their threads)
+    for (long long row0 = first, base = G == 32 ? first : first - group * R; base < a.rows; row0 += step, base += step) {
+        const int left = (int)(a.rows - row0 < R ? a.rows - row0 : R);
+        Vals<V> d[R][ITEMS];
+        float x0[R], shift[R], rstd[R];
+        if constexpr (ASYNC) {
+            fetch(stage == 0 ? STAGES - 1 : stage - 1);
+            copy_commit();
+            copy_wait<STAGES - 1>();
+        }
+        // (rows past the last are computed on whatever the ring holds, and not stored)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            Pack<T, V> x[ITEMS];
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                if (k >= FULL && k * G >= mine) continue;
+                if constexpr (ASYNC) x[k] = *slot(stage, r, k);
+                else if (r < left) x[k] = *reinterpret_cast<const Pack<T, V>*>(now + r * x_row + k * (G * PACK));
+            }
+            if constexpr (G > 32) x0[r] = next[r];
+            else x0[r] = __shfl_sync(0xffffffffu, to_f(x[0].v[0]), 0, G);
+            Vals<V> sum = splat<V>(0.f);
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                if (k >= FULL && k * G >= mine) continue;
+                d[r][k] = sub(to_vals<T, V>(x[k]), splat<V>(x0[r]));
+                sum = add(sum, d[r][k]);
+            }
+            shift[r] = total(sum);
+        }
+        now += step * x_row;
+        fetch_first(a.rows - row0 - step);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        group_sum<G, R>(shift, s_red, 0);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            shift[r] *= inv_d;
+            Vals<V> sq = splat<V>(0.f);
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                if (k >= FULL && k * G >= mine) continue;
+                d[r][k] = sub(d[r][k], splat<V>(shift[r]));
+                sq = fma(d[r][k], d[r][k], sq);
+            }
+            rstd[r] = total(sq);
+        }
+        group_sum<G, R>(rstd, s_red, 1);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            rstd[r] = rsqrtf(rstd[r] * inv_d + a.eps);
+            if (lane == 0 && a.stats && r < left) a.stats[row0 + r] = RowStats{x0[r], shift[r], rstd[r], 0.f};
+        }
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) {
+            if (k >= FULL && k * G >= mine) continue;
+            const Vals<V> w = staged_weights<V>(s_w, k * G + lane, packs), b = staged_weights<V>(s_b, k * G + lane, packs);
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (r < left)
+                    *reinterpret_cast<Pack<T, V>*>(out + r * y_row + k * (G * PACK)) =
+                        to_pack<T, V>(fma(mul(d[r][k], splat<V>(rstd[r])), w, b));
+        }
+        out += step * y_row;
+    }
+    if constexpr (ASYNC) copy_wait<0>();
 }
 
 // Rows of any width: one CTA per row, the row read three times (from L2 after the first).
@@ -125,52 +248,62 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_any_kernel(NormArgs a) 
             const float d = (to_f(x[c]) - x0) - shift;
             sq = fmaf(d, d, sq);
         }
-        const float rstd = 1.f / sqrtf(block_sum_all(sq, s_red, 1) * inv_d + a.eps);
+        const float rstd = rsqrtf(block_sum_all(sq, s_red, 1) * inv_d + a.eps);
         for (long long c = threadIdx.x; c < a.D; c += LN_THREADS) {
             const float xhat = ((to_f(x[c]) - x0) - shift) * rstd;
             y[c] = from_f<T>(fmaf(xhat, w ? to_f(w[c]) : 1.f, b ? to_f(b[c]) : 0.f));
         }
-        if (threadIdx.x == 0 && a.shift) {
-            a.shift[r] = shift;
-            a.rstd[r] = rstd;
-        }
+        if (threadIdx.x == 0 && a.stats) a.stats[r] = RowStats{x0, shift, rstd, 0.f};
     }
 }
 
-// Calls f(G, ITEMS, R) with the narrowest group of threads that holds `packs` packs of V values: a warp
-// where 32 values a thread do (sums without a barrier), else up to 1024 threads; false when none does.
+// Calls f(G, ITEMS, R) with the narrowest group of threads that holds `packs` packs of V values, false when
+// none does.  Few rows: at most 16 values a thread, up to 1024 threads.
 template <int V, typename F>
 static bool with_norm_group(long long packs, F&& f) {
-    constexpr int I = V == 1 ? 16 : 32 / V;  // packs a thread of a wide group
-    if (packs <= 8) f(Int<8>{}, Int<1>{}, Int<2>{});
-    else if (packs <= 32) f(Int<32>{}, Int<1>{}, Int<4>{});
-    else if (packs <= 32 * (8 / (V < 8 ? V : 8)) && V < 8) f(Int<32>{}, Int<8 / (V < 8 ? V : 8)>{}, Int<2>{});
-    else if (packs <= 32 * (16 / V)) f(Int<32>{}, Int<16 / V>{}, Int<2>{});
-    else if (packs <= 32 * (32 / V)) f(Int<32>{}, Int<32 / V>{}, Int<1>{});
-    else if (packs <= 128 * I) f(Int<128>{}, Int<I>{}, Int<1>{});
-    else if (packs <= 256 * I) f(Int<256>{}, Int<I>{}, Int<1>{});
+    constexpr int I = 16 / V, H = (I + 1) / 2;  // packs a thread, half of them
+    if (packs <= 8) f(Int<8>{}, Int<1>{}, Int<1>{});
+    else if (packs <= 32) f(Int<32>{}, Int<1>{}, Int<1>{});
+    else if (packs <= 128 * H) f(Int<128>{}, Int<H>{}, Int<1>{});
+    else if (packs <= 256 * H) f(Int<256>{}, Int<H>{}, Int<1>{});
+    else if (packs <= 512 * H) f(Int<512>{}, Int<H>{}, Int<1>{});
     else if (packs <= 512 * I) f(Int<512>{}, Int<I>{}, Int<1>{});
     else if (packs <= 1024 * I) f(Int<1024>{}, Int<I>{}, Int<1>{});
     else return false;
     return true;
 }
-
 template <typename T, typename W, int V>
-static bool launch_norm_packs(const NormArgs& a, cudaStream_t s) {
-    return with_norm_group<V>(a.D / V, [&](auto g, auto items, auto r) {
-        constexpr int G = decltype(g)::value, ITEMS = decltype(items)::value, R = decltype(r)::value;
+static bool launch_norm_packs(const NormArgs& a, int device, cudaStream_t s) {
+    // Rows stream once every SM has several to keep its blocks busy.
+    if (a.rows >= 8ll * sm_count(device)) {
+        const bool done = with_stream_group<T, V>(a.D / V, [&](auto g, auto items, auto full) {
+            constexpr int G = decltype(g)::value, ITEMS = decltype(items)::value, FULL = decltype(full)::value;
+            constexpr int R = G >= 256 ? 2 : ITEMS * V <= 16 ? 4 : 2;  // 64 values a thread in registers
+            constexpr int BLOCK = norm_block(G), PER = BLOCK / G * R;
+            constexpr size_t ring = norm_async<T, V> ? sizeof(Pack<T, V>) * norm_stages<T, V>(ITEMS * R, BLOCK) * R * ITEMS * BLOCK : 0;
+            constexpr size_t most = ring + (size_t)BLOCK / (BLOCK / G) * ITEMS * V * 2 * sizeof(float);  // (of the widest row)
+            static int cached[64];
+            const auto kernel = layer_norm_stream_kernel<T, W, V, G, ITEMS, FULL, R>;
+            const long long resident = (long long)blocks_per_sm(kernel, BLOCK, most, device, cached) * sm_count(device);
+            const long long batches = (a.rows + PER - 1) / PER;
+            kernel<<<(unsigned)(batches < resident ? batches : resident), BLOCK, ring + (size_t)a.D * 2 * sizeof(float), s>>>(a);
+        });
+        if (done) return true;
+    }
+    return with_norm_group<V>(a.D / V, [&](auto g, auto items, auto rr) {
+        constexpr int G = decltype(g)::value, ITEMS = decltype(items)::value, R = decltype(rr)::value;
         constexpr int PER = norm_block(G) / G * R;
         layer_norm_kernel<T, W, V, G, ITEMS, R><<<row_grid((a.rows + PER - 1) / PER), norm_block(G), 0, s>>>(a);
     });
 }
 
 template <typename T, typename W>
-static void launch_norm(const NormArgs& a, cudaStream_t s) {
+static void launch_norm(const NormArgs& a, int device, cudaStream_t s) {
     const int bytes = norm_pack_bytes(a.x, a.y, nullptr, a.w, a.b, a.D, a.row_stride, sizeof(T), sizeof(W));
     bool done = false;
-    if (bytes == 16) done = launch_norm_packs<T, W, 16 / sizeof(T)>(a, s);
-    else if (bytes == 4) done = launch_norm_packs<T, W, 4 / sizeof(T)>(a, s);
-    else done = launch_norm_packs<T, W, 1>(a, s);
+    if (bytes == 16) done = launch_norm_packs<T, W, 16 / sizeof(T)>(a, device, s);
+    else if (bytes == 4) done = launch_norm_packs<T, W, 4 / sizeof(T)>(a, device, s);
+    else done = launch_norm_packs<T, W, 1>(a, device, s);
     if (!done) layer_norm_any_kernel<T, W><<<row_grid(a.rows), LN_THREADS, 0, s>>>(a);
 }
 
@@ -179,21 +312,21 @@ static void launch_norm(const NormArgs& a, cudaStream_t s) {
 using namespace igs;
 
 extern "C" int igs_layer_norm(const void* x, int dtype, long long rows, long long D, long long row_stride,
-                              const void* weight, const void* bias, int wdtype, float eps, void* y, float* shift,
-                              float* rstd, int device, void* stream) {
+                              const void* weight, const void* bias, int wdtype, float eps, void* y, float* stats,
+                              int device, void* stream) {
     const int rc = norm_args_ok(rows, D, row_stride, dtype, wdtype);
     if (rc) return rc;
-    if (!(eps >= 0.f) || (!shift != !rstd)) return IGS_ERR_ARG;
+    if (!(eps >= 0.f) || !aligned_to(stats, 16)) return IGS_ERR_ARG;
     if (rows == 0) return IGS_OK;
     if (!x || !y) return IGS_ERR_ARG;
     DeviceGuard guard(device);
     if (!guard.ok) return IGS_ERR_DEVICE;
     cudaStream_t s = (cudaStream_t)stream;
-    NormArgs a{x, weight, bias, y, shift, rstd, rows, D, row_stride, eps};
+    NormArgs a{x, weight, bias, y, reinterpret_cast<RowStats*>(stats), rows, D, row_stride, eps};
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        if (wdtype == dtype) launch_norm<T, T>(a, s);
-        else launch_norm<T, float>(a, s);
+        if (wdtype == dtype) launch_norm<T, T>(a, device, s);
+        else launch_norm<T, float>(a, device, s);
         return 0;
     });
     count_launch();

@@ -5,18 +5,17 @@
 
 namespace igs {
 
-// V weights as floats; without any, the value they stand for
+// What the gradient needs of a row, one 16-byte load: its first value, mean - first value, rstd.
+struct alignas(16) RowStats {
+    float x0, shift, rstd, unused;
+};
+
+// V weights; without any, the value they stand for
 template <typename W, int V>
-__device__ __forceinline__ void load_weights(const void* w, long long c, float none, float (&out)[V]) {
-    if (!w) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) out[j] = none;
-        return;
-    }
+__device__ __forceinline__ Vals<V> load_weights(const void* w, int pack, float none) {
+    if (!w) return splat<V>(none);
     // (a pack may be longer than the 16 bytes that one load moves)
-    const Pack<W, V> p = *reinterpret_cast<const Pack<W, V>*>(static_cast<const W*>(w) + c);
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = to_f(p.v[j]);
+    return to_vals<W, V>(static_cast<const Pack<W, V>*>(w)[pack]);
 }
 
 __host__ __device__ constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
@@ -69,13 +68,68 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* s_red, int turn)
     }
 }
 
-// Threads of a block whose groups have G threads
-__host__ __device__ constexpr int norm_block(int G) { return G < 128 ? 128 : G; }
+// Threads of a block whose groups have G threads: four warps, or one wider group
+__host__ __device__ constexpr int norm_block(int G) { return G <= 32 ? 128 : G; }
+// Blocks that an SM is to hold: 384 threads with 168 registers each
+__host__ __device__ constexpr int norm_blocks(int G) { return norm_block(G) >= 256 ? 1 : 384 / norm_block(G); }
 
+// Weights in shared memory in 32 bits, as a thread reads its packs of V: the 16-byte quarters of all
+// packs in planes of their own, so that the lanes of a warp read neighbouring 16 bytes.
+template <int V>
+__device__ __forceinline__ int weight_place(int column, int packs) {
+    if constexpr (V <= 4) return column;
+    const int p = column / V, j = column % V;
+    return (j / 4) * packs * 4 + p * 4 + j % 4;
+}
+template <typename W, int V>
+__device__ __forceinline__ void stage_weights(float* s_w, const void* w, float none, int D, int packs, int block) {
+    for (int c = threadIdx.x; c < D; c += block)
+        s_w[weight_place<V>(c, packs)] = w ? to_f(static_cast<const W*>(w)[c]) : none;
+}
+template <int V>
+__device__ __forceinline__ Vals<V> staged_weights(const float* s_w, int pack, int packs) {
+    if constexpr (V <= 4) return to_vals<float, V>(reinterpret_cast<const Pack<float, V>*>(s_w)[pack]);
+    else {
+        Vals<V> r;
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+            const Vals<4> t = to_vals<float, 4>(reinterpret_cast<const Pack<float, 4>*>(s_w)[q * packs + pack]);
+            r.v[2 * q] = t.v[0];
+            r.v[2 * q + 1] = t.v[1];
+        }
+        return r;
+    }
+}
+
+// Calls f(G, ITEMS, FULL) with the narrowest group of threads that holds `packs` packs of V values of T,
+// false when none does: up to 32 values a thread of 16-bit types, 16 of 32-bit ones (the same bytes in
+// flight a thread).  As few threads a row as possible, since what a row costs beside its values (two
+// sums across its threads, addresses, its statistics) is paid per thread.  The first FULL items are
+// there in every thread: a check per item costs registers and moves (all items checked, the gradient
+// of 65536 x 1024 bf16 took 88 us instead of 71).
 template <int N>
 struct Int {
     static constexpr int value = N;
 };
+template <typename T, int V, typename F>
+inline bool with_stream_group(long long packs, F&& f) {
+    constexpr int J = 16 / V, I = sizeof(T) == 2 && V > 1 ? 2 * J : J;  // the most packs a thread
+    constexpr int Q = I / 4, H = I / 2;
+    if (packs <= 8) f(Int<8>{}, Int<1>{}, Int<0>{});
+    else if (packs <= 32) f(Int<32>{}, Int<1>{}, Int<0>{});
+    else if (Q > 1 && packs <= 32 * Q) f(Int<32>{}, Int<Q>{}, Int<1>{});
+    else if (packs <= 32 * H) f(Int<32>{}, Int<H>{}, Int<Q>{});
+    else if (packs <= 32 * (H + Q)) f(Int<32>{}, Int<H + Q>{}, Int<H>{});
+    else if (packs <= 32 * I) f(Int<32>{}, Int<I>{}, Int<H + Q>{});
+    else if (packs <= 64 * (H + Q)) f(Int<64>{}, Int<H + Q>{}, Int<H>{});
+    else if (packs <= 64 * I) f(Int<64>{}, Int<I>{}, Int<H + Q>{});
+    else if (packs <= 128 * (H + Q)) f(Int<128>{}, Int<H + Q>{}, Int<H>{});
+    else if (packs <= 128 * I) f(Int<128>{}, Int<I>{}, Int<H + Q>{});
+    else if (I == J && packs <= 256 * J) f(Int<256>{}, Int<J>{}, Int<J / 2>{});
+    else if (packs <= 512 * J) f(Int<512>{}, Int<J>{}, Int<J / 2>{});
+    else return false;
+    return true;
+}
 
 // The pack sizes in bytes that the kernels move, the widest that fits: every row of x, y (dy, dx)
 // and the weights start on one.
@@ -88,6 +142,47 @@ inline int norm_pack_bytes(const void* x, const void* y, const void* z, const vo
             return (int)bytes;
     }
     return (int)tsize;
+}
+
+// What a thread copies ahead: PACK bytes of 4 or 16.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+// 16-bit values one by one cannot be copied that way.
+template <typename T, int V>
+constexpr bool norm_async = sizeof(Pack<T, V>) >= 4;
+// Batches in a thread's ring of copies, the one being worked on included, when a batch is `packs` packs
+// a thread: as many as fit 384 bytes a thread (256 in blocks of 512, whose weights take up to 64 KB of
+// shared memory), two to four.
+template <typename T, int V>
+__host__ __device__ constexpr int norm_stages(int packs, int block) {
+    const int n = (block < 512 ? 384 : 256) / (int)(sizeof(Pack<T, V>) * packs);
+    return n < 2 ? 2 : n > 4 ? 4 : n;
+}
+
+// Blocks of a kernel that an SM holds, found once per device; the first call also allows the kernel
+// its shared memory.
+template <typename K>
+inline int blocks_per_sm(K kernel, int block, size_t smem, int device, int (&cached)[64]) {
+    if (device >= 0 && device < 64 && cached[device]) return cached[device];
+    int n = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, block, smem) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        n = 1;
+    }
+    if (device >= 0 && device < 64) cached[device] = n;
+    return n;
 }
 
 inline int norm_args_ok(long long rows, long long D, long long row_stride, int dtype, int wdtype) {

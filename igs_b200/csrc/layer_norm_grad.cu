@@ -14,8 +14,7 @@ struct NormGradArgs {
     const void* dy;
     const void* x;
     const void* w;
-    const float* shift;
-    const float* rstd;
+    const RowStats* stats;
     void* dx;         // NULL: not wanted
     void* dw;
     void* db;
@@ -25,168 +24,147 @@ struct NormGradArgs {
 };
 
 
-// What a thread copies ahead: PACK bytes of 4 or 16.
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src) {
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
-}
-
-// 16-bit values one by one cannot be copied that way.
-template <typename T, int V>
-constexpr bool norm_async = sizeof(Pack<T, V>) >= 4;
-// Batches of R rows in the ring, the one being worked on included: as many as fit 384 bytes a thread,
-// two to four.
-template <typename T, int V>
-__host__ __device__ constexpr int norm_stages(int items, int r) {
-    const int n = 384 / (int)(sizeof(Pack<T, V>) * 2 * items * r);
-    return n < 2 ? 2 : n > 4 ? 4 : n;
-}
-
 // Block b takes the batches b, b + gridDim.x, ... of GROUPS * R rows; ITEMS packs of V values a thread,
 // the same columns in every row.  Its groups' column sums are added in order at the end and written
 // as partial b.
-template <typename T, typename W, int V, int G, int ITEMS, int R>
-__global__ void __launch_bounds__(norm_block(G)) layer_norm_grad_kernel(NormGradArgs a) {
+template <typename T, typename W, int V, int G, int ITEMS, int FULL, int R>
+__global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad_kernel(NormGradArgs a) {
     constexpr int BLOCK = norm_block(G), GROUPS = BLOCK / G;
     constexpr int COLS = G * ITEMS * V;  // columns a group covers
     constexpr bool ASYNC = norm_async<T, V>;
-    constexpr int STAGES = norm_stages<T, V>(ITEMS, R);
+    constexpr int STAGES = norm_stages<T, V>(2 * ITEMS * R, BLOCK);
     extern __shared__ __align__(16) unsigned char s_mem[];
     __shared__ float s_red[G > 32 ? 2 * (G / 32) * 2 * R : 1];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float inv_d = 1.f / (float)a.D;
-    const int packs = (int)(a.D / V);
+    const int packs = (int)(a.D / V), mine = packs - lane;  // (item k is there when k G < mine)
     const long long step = (long long)gridDim.x * (GROUPS * R);
 
-    float w[ITEMS][V], dw[ITEMS][V], db[ITEMS][V];
+    Vals<V> dw[ITEMS], db[ITEMS];
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) w[k][j] = dw[k][j] = db[k][j] = 0.f;
-        if (k * G + lane < packs) load_weights<W, V>(a.w, (long long)(k * G + lane) * V, 1.f, w[k]);
-    }
+    for (int k = 0; k < ITEMS; ++k) dw[k] = db[k] = splat<V>(0.f);
 
-    // slot [stage][row][x or dy][item][thread]
+    // shared memory: the ring, slot [stage][row][x or dy][item][thread]; then the weights
+    constexpr int PACK = sizeof(Pack<T, V>);
+    float* s_w = reinterpret_cast<float*>(s_mem + (ASYNC ? STAGES * R * 2 * ITEMS * BLOCK * PACK : 0));
     Pack<T, V>* ring = reinterpret_cast<Pack<T, V>*>(s_mem) + threadIdx.x;
     const auto slot = [&](int stage, int r, int which, int k) {
         return ring + ((stage * R + r) * 2 + which) * ITEMS * BLOCK + k * BLOCK;
     };
-    const auto fetch = [&](long long row0, int stage) {
+    // (addresses advance by a fixed number of bytes: this thread's first pack of a batch's first row)
+    const long long first = (long long)blockIdx.x * (GROUPS * R) + group * R;
+    const long long x_row = a.row_stride * (long long)sizeof(T), y_row = a.D * (long long)sizeof(T);
+    const char* x_ahead = static_cast<const char*>(a.x) + first * x_row + lane * PACK;
+    const char* dy_ahead = static_cast<const char*>(a.dy) + first * y_row + lane * PACK;
+    const char *x_now = x_ahead, *dy_now = dy_ahead;  // (used where nothing is copied ahead)
+    char* out = static_cast<char*>(a.dx) + first * y_row + lane * PACK;
+    long long ahead_left = a.rows - first;
+    const auto fetch = [&](int stage) {
+        const int n = (int)(ahead_left < R ? ahead_left : R);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (row0 + r >= a.rows) continue;
-            const Pack<T, V>* xs = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.x) + (row0 + r) * a.row_stride);
-            const Pack<T, V>* ds = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.dy) + (row0 + r) * a.D);
+            if (r >= n) break;
 #pragma unroll
             for (int k = 0; k < ITEMS; ++k) {
-                if (k * G + lane >= packs) continue;
-                copy_async<sizeof(Pack<T, V>)>(slot(stage, r, 0, k), xs + k * G + lane);
-                copy_async<sizeof(Pack<T, V>)>(slot(stage, r, 1, k), ds + k * G + lane);
+                if (k >= FULL && k * G >= mine) continue;
+                copy_async<PACK>(slot(stage, r, 0, k), x_ahead + r * x_row + k * (G * PACK));
+                copy_async<PACK>(slot(stage, r, 1, k), dy_ahead + r * y_row + k * (G * PACK));
             }
         }
+        x_ahead += step * x_row;
+        dy_ahead += step * y_row;
+        ahead_left -= step;
     };
-
-    const long long first = (long long)blockIdx.x * (GROUPS * R) + group * R;
     if constexpr (ASYNC) {
 #pragma unroll
         for (int q = 0; q < STAGES - 1; ++q) {
-            fetch(first + q * step, q);
+            fetch(q);
             copy_commit();
         }
     }
-    // (the three numbers of a row are loaded one batch ahead)
-    float next_x0[R], next_shift[R], next_rstd[R];
-    const auto fetch_row = [&](long long row0) {
+    // (a row's statistics are loaded one batch ahead; a row past the last has a factor of zero)
+    RowStats next[R];
+    const RowStats* stats = a.stats + first;
+    const auto fetch_stats = [&](long long rows_left) {
+        const int n = (int)(rows_left < R ? rows_left : R);
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const bool ok = row0 + r < a.rows;
-            next_x0[r] = ok ? to_f(static_cast<const T*>(a.x)[(row0 + r) * a.row_stride]) : 0.f;
-            next_shift[r] = ok ? a.shift[row0 + r] : 0.f;
-            next_rstd[r] = ok ? a.rstd[row0 + r] : 0.f;
-        }
+        for (int r = 0; r < R; ++r) next[r] = r < n ? stats[r] : RowStats{0.f, 0.f, 0.f, 0.f};
+        stats += step;
     };
-    fetch_row(first);
+    fetch_stats(a.rows - first);
+    stage_weights<W, V>(s_w, a.w, 1.f, (int)a.D, packs, BLOCK);
+    __syncthreads();
 
     int turn = 0, stage = 0;
-    // (every group of a block makes the same number of steps: a barrier is met by all of its threads)
-    for (long long row0 = first, base = first - group * R; base < a.rows; row0 += step, base += step) {
-        Pack<T, V> x[R][ITEMS], dy[R][ITEMS];
-        float x0[R], shift[R], rstd[R], s[2 * R];
+    // (a warp goes on while it has a row; narrower groups share one and go on together, a wider group
+    // is the block: barriers and exchanges are met by all of their threads)
+    for (long long row0 = first, base = G == 32 ? first : first - group * R; base < a.rows; row0 += step, base += step) {
+        const int left = (int)(a.rows - row0 < R ? a.rows - row0 : R);
+        Vals<V> xh[R][ITEMS], g[R][ITEMS];  // xhat and dy w
+        float rstd[R], s[2 * R];
         if constexpr (ASYNC) {
-            fetch(row0 + (STAGES - 1) * step, (stage + STAGES - 1) % STAGES);
+            fetch(stage == 0 ? STAGES - 1 : stage - 1);
             copy_commit();
             copy_wait<STAGES - 1>();
         }
+        Vals<V> s1[R], s2[R], x0[R], f[R], t[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            x0[r] = next_x0[r];
-            shift[r] = next_shift[r];
-            rstd[r] = next_rstd[r];
+            rstd[r] = next[r].rstd;
+            s1[r] = s2[r] = splat<V>(0.f);
+            x0[r] = splat<V>(next[r].x0);  // xhat = (x - x0) rstd - shift rstd
+            f[r] = splat<V>(rstd[r]);
+            t[r] = splat<V>(-next[r].shift * rstd[r]);
+        }
 #pragma unroll
-            for (int k = 0; k < ITEMS; ++k) {
-                const int p = k * G + lane;
-                if (row0 + r < a.rows && p < packs) {
-                    if constexpr (ASYNC) {
-                        x[r][k] = *slot(stage, r, 0, k);
-                        dy[r][k] = *slot(stage, r, 1, k);
-                    } else {
-                        x[r][k] = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.x) + (row0 + r) * a.row_stride)[p];
-                        dy[r][k] = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.dy) + (row0 + r) * a.D)[p];
-                    }
-                } else {  // (a row past the last adds nothing to any sum: rstd is zero too)
+        for (int k = 0; k < ITEMS; ++k) {
+            if (k >= FULL && k * G >= mine) continue;
+            const Vals<V> w = staged_weights<V>(s_w, k * G + lane, packs);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) x[r][k].v[j] = dy[r][k].v[j] = from_f<T>(0.f);
+            for (int r = 0; r < R; ++r) {
+                if ((R > 1 || G < 32) && r >= left) continue;
+                Pack<T, V> px, pd;
+                if constexpr (ASYNC) {
+                    px = *slot(stage, r, 0, k);
+                    pd = *slot(stage, r, 1, k);
+                } else {
+                    px = *reinterpret_cast<const Pack<T, V>*>(x_now + r * x_row + k * (G * PACK));
+                    pd = *reinterpret_cast<const Pack<T, V>*>(dy_now + r * y_row + k * (G * PACK));
                 }
+                const Vals<V> d = to_vals<T, V>(pd);
+                xh[r][k] = fma(sub(to_vals<T, V>(px), x0[r]), f[r], t[r]);
+                g[r][k] = mul(d, w);
+                s1[r] = add(s1[r], g[r][k]);
+                s2[r] = fma(g[r][k], xh[r][k], s2[r]);
+                dw[k] = fma(d, xh[r][k], dw[k]);
+                db[k] = add(db[k], d);
             }
         }
-        fetch_row(row0 + step);
-        stage = (stage + 1) % STAGES;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            s[2 * r] = s[2 * r + 1] = 0.f;
-#pragma unroll
-            for (int k = 0; k < ITEMS; ++k) {
-                if (k * G + lane >= packs) continue;
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float d = to_f(dy[r][k].v[j]), xhat = ((to_f(x[r][k].v[j]) - x0[r]) - shift[r]) * rstd[r];
-                    const float g = d * w[k][j];
-                    s[2 * r] += g;
-                    s[2 * r + 1] = fmaf(g, xhat, s[2 * r + 1]);
-                    dw[k][j] = fmaf(d, xhat, dw[k][j]);
-                    db[k][j] += d;
-                }
-            }
+            s[2 * r] = total(s1[r]);
+            s[2 * r + 1] = total(s2[r]);
         }
+        x_now += step * x_row;
+        dy_now += step * y_row;
+        fetch_stats(a.rows - row0 - step);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
         if (a.dx) {  // (the same for every thread)
             group_sum<G, 2 * R>(s, s_red, turn);
             turn ^= 1;
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                if (row0 + r >= a.rows) continue;
-                const float m1 = s[2 * r] * inv_d, m2 = s[2 * r + 1] * inv_d;
-                T* out = static_cast<T*>(a.dx) + (row0 + r) * a.D;
+                if (r >= left) continue;
+                // rstd (g - m1 - xhat m2)
+                const Vals<V> c1 = splat<V>(-(s[2 * r] * inv_d) * rstd[r]), c2 = splat<V>(-(s[2 * r + 1] * inv_d) * rstd[r]);
 #pragma unroll
                 for (int k = 0; k < ITEMS; ++k) {
-                    const int p = k * G + lane;
-                    if (p >= packs) continue;
-                    Pack<T, V> o;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const float xhat = ((to_f(x[r][k].v[j]) - x0[r]) - shift[r]) * rstd[r];
-                        o.v[j] = from_f<T>(rstd[r] * (to_f(dy[r][k].v[j]) * w[k][j] - m1 - xhat * m2));
-                    }
-                    reinterpret_cast<Pack<T, V>*>(out)[p] = o;
+                    if (k >= FULL && k * G >= mine) continue;
+                    *reinterpret_cast<Pack<T, V>*>(out + r * y_row + k * (G * PACK)) =
+                        to_pack<T, V>(fma(xh[r][k], c2, fma(g[r][k], f[r], c1)));
                 }
             }
+            out += step * y_row;
         }
     }
 
@@ -197,12 +175,14 @@ __global__ void __launch_bounds__(norm_block(G)) layer_norm_grad_kernel(NormGrad
         float* s_cols = reinterpret_cast<float*>(s_mem);  // [group][dw, db][columns], over the ring
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < ITEMS; ++k)
+        for (int k = 0; k < ITEMS; ++k) {
+            const Pack<float, V> pw = to_pack<float, V>(dw[k]), pb = to_pack<float, V>(db[k]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                s_cols[(group * 2) * COLS + (k * G + lane) * V + j] = dw[k][j];
-                s_cols[(group * 2 + 1) * COLS + (k * G + lane) * V + j] = db[k][j];
+                s_cols[(group * 2) * COLS + (k * G + lane) * V + j] = pw.v[j];
+                s_cols[(group * 2 + 1) * COLS + (k * G + lane) * V + j] = pb.v[j];
             }
+        }
         __syncthreads();
         for (int i = threadIdx.x; i < 2 * COLS; i += BLOCK) {
             const int which = i / COLS, c = i % COLS;
@@ -215,11 +195,9 @@ __global__ void __launch_bounds__(norm_block(G)) layer_norm_grad_kernel(NormGrad
         for (int k = 0; k < ITEMS; ++k) {
             const int p = k * G + lane;
             if (p >= packs) continue;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                part[(long long)p * V + j] = dw[k][j];
-                part[a.D + (long long)p * V + j] = db[k][j];
-            }
+            // (D is a multiple of V: whole packs of up to 16 bytes)
+            reinterpret_cast<Pack<float, V>*>(part)[p] = to_pack<float, V>(dw[k]);
+            reinterpret_cast<Pack<float, V>*>(part + a.D)[p] = to_pack<float, V>(db[k]);
         }
     }
 }
@@ -234,18 +212,18 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_dx_any_kernel(NormGradA
         const T* x = static_cast<const T*>(a.x) + r * a.row_stride;
         const T* dy = static_cast<const T*>(a.dy) + r * a.D;
         T* dx = static_cast<T*>(a.dx) + r * a.D;
-        const float x0 = to_f(x[0]), shift = a.shift[r], rstd = a.rstd[r];
+        const RowStats st = a.stats[r];
         float s1 = 0.f, s2 = 0.f;
         for (long long c = threadIdx.x; c < a.D; c += LN_THREADS) {
             const float g = to_f(dy[c]) * (w ? to_f(w[c]) : 1.f);
             s1 += g;
-            s2 = fmaf(g, ((to_f(x[c]) - x0) - shift) * rstd, s2);
+            s2 = fmaf(g, ((to_f(x[c]) - st.x0) - st.shift) * st.rstd, s2);
         }
         const float m1 = block_sum_all(s1, s_red, 0) * inv_d;
         const float m2 = block_sum_all(s2, s_red, 1) * inv_d;
         for (long long c = threadIdx.x; c < a.D; c += LN_THREADS) {
             const float g = to_f(dy[c]) * (w ? to_f(w[c]) : 1.f);
-            dx[c] = from_f<T>(rstd * (g - m1 - ((to_f(x[c]) - x0) - shift) * rstd * m2));
+            dx[c] = from_f<T>(st.rstd * (g - m1 - ((to_f(x[c]) - st.x0) - st.shift) * st.rstd * m2));
         }
     }
 }
@@ -262,8 +240,8 @@ __global__ void __launch_bounds__(32 * LN_COL_ROWS) layer_norm_columns_kernel(No
     if (c < a.D) {
         for (long long r = lo + threadIdx.y; r < hi; r += LN_COL_ROWS) {
             const float dy = to_f(static_cast<const T*>(a.dy)[r * a.D + c]);
-            const T* x = static_cast<const T*>(a.x) + r * a.row_stride;
-            sw = fmaf(dy, ((to_f(x[c]) - to_f(x[0])) - a.shift[r]) * a.rstd[r], sw);
+            const RowStats st = a.stats[r];
+            sw = fmaf(dy, ((to_f(static_cast<const T*>(a.x)[r * a.row_stride + c]) - st.x0) - st.shift) * st.rstd, sw);
             sb += dy;
         }
     }
@@ -314,48 +292,20 @@ static int norm_splits(long long rows, long long D, int sms) {
     return (int)(rows < most ? rows : most);
 }
 
-// Calls f(G, ITEMS, R) with the narrowest group of threads that holds `packs` packs of V values, at most
-// 16 values a thread (their weights and column sums take 48 registers); false when none does.
-template <int V, typename F>
-static bool with_norm_grad_group(long long packs, F&& f) {
-    constexpr int I = 16 / V, H = (I + 1) / 2;  // packs a thread, half of them
-    if (packs <= 8) f(Int<8>{}, Int<1>{}, Int<2>{});
-    else if (packs <= 32) f(Int<32>{}, Int<1>{}, Int<2>{});
-    else if (packs <= 128 * H) f(Int<128>{}, Int<H>{}, Int<2>{});
-    else if (packs <= 128 * I) f(Int<128>{}, Int<I>{}, Int<2>{});
-    else if (packs <= 256 * I) f(Int<256>{}, Int<I>{}, Int<1>{});
-    else if (packs <= 512 * I) f(Int<512>{}, Int<I>{}, Int<1>{});
-    else return false;
-    return true;
-}
-
-// Blocks of a kernel that an SM holds, found once per device; the first call also allows the kernel
-// its shared memory.
-template <typename K>
-static int blocks_per_sm(K kernel, int block, size_t smem, int device, int (&cached)[64]) {
-    if (device >= 0 && device < 64 && cached[device]) return cached[device];
-    int n = 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, block, smem) != cudaSuccess || n <= 0) {
-        cudaGetLastError();
-        n = 1;
-    }
-    if (device >= 0 && device < 64) cached[device] = n;
-    return n;
-}
-
 // `a.splits` comes in as the most blocks and goes out as the blocks that wrote partial sums
 template <typename T, typename W, int V>
 static bool launch_norm_grad_packs(NormGradArgs& a, int device, cudaStream_t s) {
-    return with_norm_grad_group<V>(a.D / V, [&](auto g, auto items, auto rr) {
-        constexpr int G = decltype(g)::value, ITEMS = decltype(items)::value, R = decltype(rr)::value;
+    return with_stream_group<T, V>(a.D / V, [&](auto g, auto items, auto full) {
+        constexpr int G = decltype(g)::value, ITEMS = decltype(items)::value, FULL = decltype(full)::value;
+        constexpr int R = G >= 512 ? 1 : ITEMS * V <= 8 ? 4 : ITEMS * V <= 16 ? 2 : 1;  // 64 values a thread in registers, xhat and dy w
         constexpr int BLOCK = norm_block(G), PER = BLOCK / G * R;
-        constexpr size_t ring = norm_async<T, V> ? sizeof(Pack<T, V>) * norm_stages<T, V>(ITEMS, R) * R * 2 * ITEMS * BLOCK : 0;
+        constexpr size_t ring = norm_async<T, V> ? sizeof(Pack<T, V>) * norm_stages<T, V>(2 * ITEMS * R, BLOCK) * R * 2 * ITEMS * BLOCK : 0;
         constexpr size_t cols = BLOCK > G ? (size_t)BLOCK * ITEMS * V * 2 * sizeof(float) : 0;
-        constexpr size_t smem = ring > cols ? ring : cols;
+        constexpr size_t widest = ring + (size_t)G * ITEMS * V * sizeof(float), most = widest > cols ? widest : cols;
+        const size_t used = ring + (size_t)a.D * sizeof(float), smem = used > cols ? used : cols;
         static int cached[64];
-        const auto kernel = layer_norm_grad_kernel<T, W, V, G, ITEMS, R>;
-        const long long resident = (long long)blocks_per_sm(kernel, BLOCK, smem, device, cached) * sm_count(device);
+        const auto kernel = layer_norm_grad_kernel<T, W, V, G, ITEMS, FULL, R>;
+        const long long resident = (long long)blocks_per_sm(kernel, BLOCK, most, device, cached) * sm_count(device);
         const long long batches = (a.rows + PER - 1) / PER;
         if (resident < a.splits) a.splits = (int)resident;
         if (batches < a.splits) a.splits = (int)batches;
@@ -399,13 +349,13 @@ extern "C" size_t igs_layer_norm_grad_workspace_bytes(long long rows, long long 
 }
 
 extern "C" int igs_layer_norm_grad(const void* dy, const void* x, int dtype, long long rows, long long D,
-                                   long long row_stride, const void* weight, int wdtype, const float* shift,
-                                   const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                                   long long row_stride, const void* weight, int wdtype, const float* stats,
+                                   void* dx, void* dweight, void* dbias, void* workspace,
                                    size_t workspace_bytes, int device, void* stream) {
     const int rc = norm_args_ok(rows, D, row_stride, dtype, wdtype);
     if (rc) return rc;
     const size_t wsize = dtype_size(wdtype);
-    if (rows > 0 && (!dy || !x || !shift || !rstd)) return IGS_ERR_ARG;
+    if (rows > 0 && (!dy || !x || !stats || !aligned_to(stats, 16))) return IGS_ERR_ARG;
     const bool columns = dweight || dbias;
     if (rows > 0 && columns && (!workspace || workspace_bytes < igs_layer_norm_grad_workspace_bytes(rows, D, device)))
         return IGS_ERR_WORKSPACE;
@@ -419,7 +369,7 @@ extern "C" int igs_layer_norm_grad(const void* dy, const void* x, int dtype, lon
         return (int)e;
     }
     if (!dx && !columns) return IGS_OK;
-    NormGradArgs a{dy, x, weight, shift, rstd, dx, dweight, dbias, static_cast<float*>(workspace), rows, D, row_stride,
+    NormGradArgs a{dy, x, weight, reinterpret_cast<const RowStats*>(stats), dx, dweight, dbias, static_cast<float*>(workspace), rows, D, row_stride,
                    norm_splits(rows, D, sm_count(device))};
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);

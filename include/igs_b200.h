@@ -429,13 +429,13 @@ int igs_embed_grad(const void* tokens, int token_bytes, long long n, const void*
  * Layer norm over rows of D values: y = (x - mean) * rstd * weight + bias, rstd =
  * 1 / sqrt(var + eps) with the biased variance.  x [rows,D] with `row_stride` elements between
  * rows, y [rows,D] contiguous; weight, bias [D] of type wdtype (x's type or IGS_F32) or NULL
- * for ones / zeros.  shift, rstd [rows] (fp32) are what the gradient needs; both NULL when it is
- * not wanted.  The mean is kept as its distance from the row's first value, mean = x[0] + shift,
- * so that rows far from zero lose nothing.
+ * for ones / zeros.  stats [rows,4] (fp32, on a 16-byte boundary) is what the gradient needs of
+ * every row, NULL when it is not wanted: x[0], mean - x[0], rstd and a spare.  The mean is kept as
+ * its distance from the row's first value so that rows far from zero lose nothing.
  */
 int igs_layer_norm(const void* x, int dtype, long long rows, long long D, long long row_stride,
-                   const void* weight, const void* bias, int wdtype, float eps, void* y, float* shift,
-                   float* rstd, int device, void* stream);
+                   const void* weight, const void* bias, int wdtype, float eps, void* y, float* stats,
+                   int device, void* stream);
 
 /*
  * Its gradient: dx [rows,D] (contiguous, x's type), dweight and dbias [D] (wdtype), each NULL
@@ -444,8 +444,8 @@ int igs_layer_norm(const void* x, int dtype, long long rows, long long D, long l
  */
 size_t igs_layer_norm_grad_workspace_bytes(long long rows, long long D, int device);
 int igs_layer_norm_grad(const void* dy, const void* x, int dtype, long long rows, long long D,
-                        long long row_stride, const void* weight, int wdtype, const float* shift,
-                        const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                        long long row_stride, const void* weight, int wdtype, const float* stats,
+                        void* dx, void* dweight, void* dbias, void* workspace,
                         size_t workspace_bytes, int device, void* stream);
 
 /*

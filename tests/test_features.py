@@ -50,18 +50,18 @@ def test_c_abi_refuses_bad_arguments_before_any_cuda_call():
         assert embed_grad(**bad) == -1, bad
     assert embed_grad(ws=None) == -2 and embed_grad(nb=16) == -2
 
-    def norm(x=one, dt=1, rows=4, D=8, stride=8, w=one, b=one, wdt=0, eps=1e-5, y=one, shift=one, rstd=one):
-        return lib.igs_layer_norm(x, dt, rows, D, stride, w, b, wdt, eps, y, shift, rstd, 0, None)
+    def norm(x=one, dt=1, rows=4, D=8, stride=8, w=one, b=one, wdt=0, eps=1e-5, y=one, stats=one):
+        return lib.igs_layer_norm(x, dt, rows, D, stride, w, b, wdt, eps, y, stats, 0, None)
 
     for bad in (dict(x=None), dict(y=None), dict(dt=9), dict(wdt=2), dict(rows=-1), dict(D=0), dict(stride=-8),
-                dict(eps=-1.0), dict(eps=float("nan")), dict(shift=None), dict(rstd=None)):
+                dict(eps=-1.0), dict(eps=float("nan")), dict(stats=ctypes.c_void_p(260))):
         assert norm(**bad) == -1, bad
     assert norm(rows=0, x=None, y=None) == 0
 
-    def norm_grad(dy=one, x=one, dt=1, rows=4, wdt=0, shift=one, rstd=one, dx=one, dw=one, db=one, ws=one, nb=1 << 30):
-        return lib.igs_layer_norm_grad(dy, x, dt, rows, 8, 8, one, wdt, shift, rstd, dx, dw, db, ws, nb, 0, None)
+    def norm_grad(dy=one, x=one, dt=1, rows=4, wdt=0, stats=one, dx=one, dw=one, db=one, ws=one, nb=1 << 30):
+        return lib.igs_layer_norm_grad(dy, x, dt, rows, 8, 8, one, wdt, stats, dx, dw, db, ws, nb, 0, None)
 
-    for bad in (dict(dy=None), dict(x=None), dict(shift=None), dict(rstd=None), dict(wdt=2), dict(rows=-1)):
+    for bad in (dict(dy=None), dict(x=None), dict(stats=None), dict(stats=ctypes.c_void_p(260)), dict(wdt=2), dict(rows=-1)):
         assert norm_grad(**bad) == -1, bad
     assert norm_grad(ws=None) == -2 and norm_grad(nb=16) == -2
 
