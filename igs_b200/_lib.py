@@ -66,7 +66,7 @@ SIGNATURES = {
     "igs_mse_loss": (_i, [_vp, _vp, ctypes.c_longlong, _vp, _vp, _sz, _i, _vp]),
     "igs_mse_grad": (_i, [_vp, _vp, ctypes.c_longlong, _vp, _vp, _i, _vp]),
     "igs_embed": (_i, [_vp, _i, _i64, _vp, _i, _i64, _i64, _i64, _f, _i, _i64, _vp, _i, _vp]),
-    "igs_embed_grad_workspace_bytes": (_i, [_i64, _i64, _i64, _i, ctypes.POINTER(_sz)]),
+    "igs_embed_grad_workspace_bytes": (_i, [_i64, _i64, _i64, _i, _i, ctypes.POINTER(_sz)]),
     "igs_embed_grad": (_i, [_vp, _i, _i64, _vp, _i, _i64, _i64, _f, _i, _i64, _vp, _vp, _sz, _i, _vp]),
     "igs_layer_norm": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _f, _vp, _vp, _i, _vp]),
     "igs_layer_norm_grad_workspace_bytes": (_sz, [_i64, _i64, _i]),

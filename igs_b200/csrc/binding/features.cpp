@@ -107,7 +107,7 @@ struct EmbedBackward : torch::autograd::Node {
         Tensor d_table = at::empty({call.rows, call.width}, dy.options());
         size_t bytes = 0;
         check("igs_embed_grad_workspace_bytes",
-              igs_embed_grad_workspace_bytes(n, call.rows, call.width, device_index(dy), &bytes));
+              igs_embed_grad_workspace_bytes(n, call.rows, call.width, type_code(dy.scalar_type()), device_index(dy), &bytes));
         Tensor ws = workspace(bytes, dy);
         check("igs_embed_grad",
               igs_embed_grad(tokens.data_ptr(), static_cast<int>(tokens.element_size()), n, dy.data_ptr(),

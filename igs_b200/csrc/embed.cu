@@ -22,7 +22,7 @@ namespace igs {
 constexpr int EMBED_THREADS = 128;
 constexpr int SORT_THREADS = 256;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
-constexpr int SORT_PER_WARP = 256;                       // places a warp ranks, 32 at a time
+constexpr int SORT_PER_WARP = 128;                       // places a warp ranks, 32 at a time
 constexpr int SORT_BLOCK = SORT_WARPS * SORT_PER_WARP;   // places a block ranks
 constexpr int SORT_MAX_BITS = 10;
 constexpr int SORT_MAX_DIGITS = 1 << SORT_MAX_BITS;
@@ -89,9 +89,8 @@ __global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(EmbedArgs a, int l
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if (i0 + r >= a.n) continue;
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[r].v[j] = from_f<T>(row[r] != NO_ROW ? to_f(v[r].v[j]) * a.scale : none[r]);
-            reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.out) + (i0 + r) * a.D)[p] = v[r];
+            const Vals<V> y = row[r] != NO_ROW ? mul(to_vals<T, V>(v[r]), splat<V>(a.scale)) : splat<V>(none[r]);
+            reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.out) + (i0 + r) * a.D)[p] = to_pack<T, V>(y);
         }
     }
 }
@@ -190,12 +189,17 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(SortArgs a) {
     __syncthreads();
     const long long count = a.keys_in ? *a.count_in : a.n;
     const long long base = (long long)blockIdx.x * SORT_BLOCK;
-    for (int j = threadIdx.x; j < SORT_BLOCK; j += SORT_THREADS) {
-        uint32_t key;
+    uint32_t key[SORT_BLOCK / SORT_THREADS];
+    bool ok[SORT_BLOCK / SORT_THREADS];
+#pragma unroll
+    for (int j = 0; j < SORT_BLOCK / SORT_THREADS; ++j) {
         int place;
-        // (integer counts: the result does not depend on the order of the adds)
-        if (sort_load(a, base + j, count, key, place)) atomicAdd(&s_hist[(key >> a.shift) & (a.digits - 1)], 1);
+        ok[j] = sort_load(a, base + j * SORT_THREADS + threadIdx.x, count, key[j], place);
     }
+#pragma unroll
+    for (int j = 0; j < SORT_BLOCK / SORT_THREADS; ++j)
+        // (integer counts: the result does not depend on the order of the adds)
+        if (ok[j]) atomicAdd(&s_hist[(key[j] >> a.shift) & (a.digits - 1)], 1);
     __syncthreads();
     for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) a.hist[(long long)d * a.n_blocks + blockIdx.x] = s_hist[d];
 }
@@ -228,6 +232,14 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(SortArgs a) {
     __shared__ int s_sum[SORT_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
+    const long long count = a.keys_in ? *a.count_in : a.n;
+    const long long base = (long long)blockIdx.x * SORT_BLOCK + (long long)warp * SORT_PER_WARP;
+    uint32_t key[SORT_PER_WARP / 32];
+    int place[SORT_PER_WARP / 32], rank[SORT_PER_WARP / 32];
+#pragma unroll
+    for (int j = 0; j < SORT_PER_WARP / 32; ++j)
+        if (!sort_load(a, base + j * 32 + lane, count, key[j], place[j])) key[j] = NO_ROW;
+
     // first slot of every digit: exclusive sums of the totals, four digits a thread
     constexpr int PER = SORT_MAX_DIGITS / SORT_THREADS;
     int t[PER], sum = 0;
@@ -244,7 +256,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(SortArgs a) {
         if (lane >= s) incl += v;
     }
     if (lane == 31) s_sum[warp] = incl;
-    for (int d = threadIdx.x; d < SORT_WARPS * SORT_MAX_DIGITS; d += SORT_THREADS) (&s_warp[0][0])[d] = 0;
+    for (int d = lane; d < a.digits; d += 32) s_warp[warp][d] = 0;
     __syncthreads();
     int run = incl - sum;
     for (int w = 0; w < warp; ++w) run += s_sum[w];
@@ -257,14 +269,9 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(SortArgs a) {
     if (a.count_out && blockIdx.x == 0 && threadIdx.x == SORT_THREADS - 1) *a.count_out = run;
 
     // rank within the warp, in order of place
-    const long long count = a.keys_in ? *a.count_in : a.n;
-    const long long base = (long long)blockIdx.x * SORT_BLOCK + (long long)warp * SORT_PER_WARP;
-    uint32_t key[SORT_PER_WARP / 32];
-    int place[SORT_PER_WARP / 32], rank[SORT_PER_WARP / 32];
 #pragma unroll
     for (int j = 0; j < SORT_PER_WARP / 32; ++j) {
-        const bool ok = sort_load(a, base + j * 32 + lane, count, key[j], place[j]);
-        if (!ok) key[j] = NO_ROW;
+        const bool ok = key[j] != NO_ROW;
         // pairs that are not there share a digit no pair has, so they match only each other
         const int d = ok ? (int)((key[j] >> a.shift) & (a.digits - 1)) : SORT_MAX_DIGITS;
         const unsigned peers = __match_any_sync(0xffffffffu, d);
@@ -315,6 +322,13 @@ struct SegmentArgs {
 };
 
 constexpr int CHUNK_STEP = 8;  // places whose rows are loaded together; chunks are multiples of it
+// Steps of rows in a thread's ring, the one being added included.  16-bit values one by one cannot be
+// copied asynchronously.
+constexpr int SEGMENT_STAGES = 3;
+template <typename T, int V>
+constexpr bool segment_async = sizeof(Pack<T, V>) >= 4;
+template <typename T, int V>
+constexpr size_t segment_smem = segment_async<T, V> ? sizeof(Pack<T, V>) * CHUNK_STEP * SEGMENT_STAGES * EMBED_THREADS : 0;
 
 // positions a chunk holds, the last one's less
 __device__ __forceinline__ long long chunk_length(long long count, int chunks) {
@@ -331,28 +345,20 @@ __device__ __forceinline__ bool has_key(const uint32_t* keys, int count, uint32_
     return lo < count && keys[lo] == row;
 }
 
-template <int V>
-__device__ __forceinline__ void store_part(float* part, const float (&sum)[V]) {
-    constexpr int Q = V < 4 ? V : 4;
-#pragma unroll
-    for (int j = 0; j < V; j += Q) {
-        Pack<float, Q> o;
-#pragma unroll
-        for (int i = 0; i < Q; ++i) o.v[i] = sum[j + i];
-        reinterpret_cast<Pack<float, Q>*>(part)[j / Q] = o;
-    }
-}
-
 // sum * scale to a row of the table
 template <typename T, int V>
-__device__ __forceinline__ void store_row(T* row, const float (&sum)[V], float scale) {
-    Pack<T, V> o;
-#pragma unroll
-    for (int j = 0; j < V; ++j) o.v[j] = from_f<T>(sum[j] * scale);
-    *reinterpret_cast<Pack<T, V>*>(row) = o;
+__device__ __forceinline__ void store_row(T* row, const Vals<V>& sum, float scale) {
+    *reinterpret_cast<Pack<T, V>*>(row) = to_pack<T, V>(mul(sum, splat<V>(scale)));
+}
+template <int V>
+__device__ __forceinline__ void store_part(float* part, const Vals<V>& sum) {
+    *reinterpret_cast<Pack<float, V>*>(part) = to_pack<float, V>(sum);
 }
 
-// grid (sum blocks + zero blocks, column slabs).  Every thread owns one pack of V columns.
+// grid (sum blocks + zero blocks, column slabs).  Every thread owns one pack of V columns and copies the
+// rows of the next steps to shared memory of its own ahead of time: rows lie anywhere in dy, and what
+// bounds the kernel is how many of them are on their way (plain loads, eight a thread between
+// additions: 85 us for 65536 rows of 1024 bf16; the ring: NEWTIME).
 template <typename T, int V>
 __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
     const int count = *a.count;
@@ -390,43 +396,85 @@ __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
     float* part = a.part + chunk * 2 * a.D + pack * V;
     const bool from_before = lo > 0 && a.keys[lo - 1] == a.keys[lo];
     const bool goes_on = hi < count && a.keys[hi] == a.keys[hi - 1];
-    uint32_t key = a.keys[lo];
-    bool first = true;
-    float sum[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] = 0.f;
-    for (long long p = lo; p < hi; p += CHUNK_STEP) {
-        // (lo is a multiple of CHUNK_STEP and the sort's arrays are padded to 256 bytes: whole packs)
-        const Pack<uint32_t, 4>* kp = reinterpret_cast<const Pack<uint32_t, 4>*>(a.keys + p);
-        const Pack<int, 4>* pp = reinterpret_cast<const Pack<int, 4>*>(a.places + p);
-        Pack<uint32_t, 4> k[CHUNK_STEP / 4];
-        Pack<T, V> v[CHUNK_STEP];
+    constexpr bool ASYNC = segment_async<T, V>;
+    extern __shared__ __align__(16) unsigned char s_mem[];
+    Pack<T, V>* ring = reinterpret_cast<Pack<T, V>*>(s_mem) + threadIdx.x;
+
+    // Keys and places of a step (lo is a multiple of CHUNK_STEP and the sort's arrays are padded to 256
+    // bytes: whole packs; what lies behind hi is not used)
+    struct Step {
+        Pack<uint32_t, 4> key[CHUNK_STEP / 4];
+        Pack<int, 4> place[CHUNK_STEP / 4];
+    };
+    const auto load_step = [&](long long p, Step& s) {
+        if (p >= hi) return;
 #pragma unroll
         for (int q = 0; q < CHUNK_STEP / 4; ++q) {
-            k[q] = kp[q];
-            const Pack<int, 4> at = pp[q];
+            s.key[q] = reinterpret_cast<const Pack<uint32_t, 4>*>(a.keys + p)[q];
+            s.place[q] = reinterpret_cast<const Pack<int, 4>*>(a.places + p)[q];
+        }
+    };
+    const auto fetch = [&](long long p, const Step& s, int stage) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (p + q * 4 + i < hi) v[q * 4 + i] = *reinterpret_cast<const Pack<T, V>*>(dy + (long long)at.v[i] * a.D);
+        for (int u = 0; u < CHUNK_STEP; ++u)
+            if (p + u < hi)
+                copy_async<sizeof(Pack<T, V>)>(ring + (stage * CHUNK_STEP + u) * EMBED_THREADS,
+                                               dy + (long long)s.place[u / 4].v[u % 4] * a.D);
+    };
+
+    // pipeline: step i is added while the rows of i + 1 and i + 2 are on their way and the places of
+    // i + 3 are loaded
+    static_assert(SEGMENT_STAGES == 3, "the pipeline below");
+    Step s0, s1, s2, s3;
+    load_step(lo, s0);
+    load_step(lo + CHUNK_STEP, s1);
+    load_step(lo + 2 * CHUNK_STEP, s2);
+    if constexpr (ASYNC) {
+        fetch(lo, s0, 0);
+        copy_commit();
+        fetch(lo + CHUNK_STEP, s1, 1);
+        copy_commit();
+    }
+    uint32_t key = s0.key[0].v[0];
+    bool first = true;
+    Vals<V> sum = splat<V>(0.f);
+    int stage = 0;
+    for (long long p = lo; p < hi; p += CHUNK_STEP) {
+        load_step(p + 3 * CHUNK_STEP, s3);
+        Pack<T, V> v[CHUNK_STEP];
+        if constexpr (ASYNC) {
+            fetch(p + 2 * CHUNK_STEP, s2, stage == 0 ? 2 : stage - 1);
+            copy_commit();
+            copy_wait<SEGMENT_STAGES - 1>();
+#pragma unroll
+            for (int u = 0; u < CHUNK_STEP; ++u)
+                if (p + u < hi) v[u] = ring[(stage * CHUNK_STEP + u) * EMBED_THREADS];
+            stage = stage == 2 ? 0 : stage + 1;
+        } else {
+#pragma unroll
+            for (int u = 0; u < CHUNK_STEP; ++u)
+                if (p + u < hi) v[u] = *reinterpret_cast<const Pack<T, V>*>(dy + (long long)s0.place[u / 4].v[u % 4] * a.D);
         }
 #pragma unroll
         for (int u = 0; u < CHUNK_STEP; ++u) {
             if (p + u >= hi) break;
-            const uint32_t ku = k[u / 4].v[u % 4];
+            const uint32_t ku = s0.key[u / 4].v[u % 4];
             if (ku != key) {  // (the same in every thread of the group)
-                if (first && from_before) store_part(part, sum);
+                if (first && from_before) store_part<V>(part, sum);
                 else store_row<T, V>(d_table + (long long)key * a.D, sum, a.scale);
                 first = false;
                 key = ku;
-#pragma unroll
-                for (int j = 0; j < V; ++j) sum[j] = 0.f;
+                sum = splat<V>(0.f);
             }
-#pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] += to_f(v[u].v[j]);
+            sum = add(sum, to_vals<T, V>(v[u]));
         }
+        s0 = s1;
+        s1 = s2;
+        s2 = s3;
     }
-    if (first && from_before) store_part(part, sum);
-    else if (goes_on) store_part(part + a.D, sum);
+    if constexpr (ASYNC) copy_wait<0>();
+    if (first && from_before) store_part<V>(part, sum);
+    else if (goes_on) store_part<V>(part + a.D, sum);
     else store_row<T, V>(d_table + (long long)key * a.D, sum, a.scale);
 }
 
@@ -442,30 +490,32 @@ constexpr int JOIN_THREADS = 256;
 constexpr int JOIN_DOWN = JOIN_THREADS / 32;
 template <typename T, int Q>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(SegmentArgs a, int short_blocks, int short_slabs) {
-    __shared__ float s_sum[JOIN_DOWN][32 * Q];
+    __shared__ Pack<float, Q> s_sum[JOIN_DOWN][32];
     const int count = *a.count;
     const long long len = chunk_length(count, a.chunks);
     // whether chunk k exists and begins with the key / in the middle of a run of it
     const auto begins = [&](long long k, uint32_t key) { return k * len < count && a.keys[k * len] == key; };
     const auto continues = [&](long long k, uint32_t key) { return k > 0 && begins(k, key) && a.keys[k * len - 1] == key; };
     T* d_table = static_cast<T*>(a.d_table);
-    float sum[Q];
+    const int lane = threadIdx.x & 31;
+    const auto head = [&](long long k, long long c) {
+        return to_vals<float, Q>(*reinterpret_cast<const Pack<float, Q>*>(a.part + k * 2 * a.D + c));
+    };
 
     if ((int)blockIdx.x < short_blocks) {
         const long long k0 = blockIdx.x / short_slabs;
         const long long c = ((long long)(blockIdx.x % short_slabs) * JOIN_THREADS + threadIdx.x) * Q;
         if ((k0 + 1) * len >= count) return;
         const uint32_t key = a.keys[(k0 + 1) * len];
+        // lane i looks at chunk k0 + 1 + i: how many chunks in a row begin with the key
+        static_assert(JOIN_SHORT < 32, "a warp looks past a short run");
+        const unsigned going = ~__ballot_sync(0xffffffffu, begins(k0 + 1 + lane, key));
+        const int heads = going ? __ffs(going) - 1 : 32;
         if (!continues(k0 + 1, key) || continues(k0, key)) return;  // nothing crosses, or it started before
-        if (begins(k0 + 1 + JOIN_SHORT, key) || c >= a.D) return;   // a long one
-        const Pack<float, Q> t = *reinterpret_cast<const Pack<float, Q>*>(a.part + (k0 * 2 + 1) * a.D + c);
-#pragma unroll
-        for (int j = 0; j < Q; ++j) sum[j] = t.v[j];
-        for (long long k = k0 + 1; begins(k, key); ++k) {
-            const Pack<float, Q> h = *reinterpret_cast<const Pack<float, Q>*>(a.part + k * 2 * a.D + c);
-#pragma unroll
-            for (int j = 0; j < Q; ++j) sum[j] += h.v[j];
-        }
+        if (heads > JOIN_SHORT || c >= a.D) return;                 // a long one
+        Vals<Q> sum = to_vals<float, Q>(*reinterpret_cast<const Pack<float, Q>*>(a.part + (k0 * 2 + 1) * a.D + c));
+#pragma unroll 4
+        for (int i = 0; i < heads; ++i) sum = add(sum, head(k0 + 1 + i, c));
         store_row<T, Q>(d_table + (long long)key * a.D + c, sum, a.scale);
         return;
     }
@@ -473,38 +523,36 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(SegmentArgs a, int s
     const long long slabs = (a.D + 32 * Q - 1) / (32 * Q);
     const long long b = blockIdx.x - short_blocks;
     const long long m = (b / slabs + 1) * JOIN_SHORT;
-    const int across = threadIdx.x & 31, down = threadIdx.x >> 5;
-    const long long c = ((b % slabs) * 32 + across) * Q;
+    const int down = threadIdx.x >> 5;
+    const long long c = ((b % slabs) * 32 + lane) * Q;
     if (m * len >= count) return;
     const uint32_t key = a.keys[m * len];
-    if (!continues(m, key)) return;
-    long long k0 = m - 1;  // back to the chunk in which the run starts
-    while (k0 > m - JOIN_SHORT && continues(k0, key)) --k0;
-    if (continues(k0, key)) return;  // the run holds an earlier multiple
-    if (!begins(k0 + 1 + JOIN_SHORT, key)) return;  // a short one
-    long long last = k0 + 1 + JOIN_SHORT, end = a.chunks;  // chunk `last` begins with the key, chunk `end` does not
+    // back to the chunk in which the run starts: lane i looks at chunk m - i
+    const unsigned stops = ~__ballot_sync(0xffffffffu, continues(m - lane, key));
+    const int back = stops ? __ffs(stops) - 1 : 32;
+    if (back == 0 || back > JOIN_SHORT) return;  // nothing crosses here, or the run holds an earlier multiple
+    const long long k0 = m - back;
+    // on to the last chunk that begins with the key, 31 probes at a time: chunk `last` does, `end` does not
+    long long last = m, end = a.chunks;
     while (end - last > 1) {
-        const long long mid = (last + end) / 2;
-        if (begins(mid, key)) last = mid; else end = mid;
+        const long long stride = (end - last + 31) / 32, at = last + (lane + 1) * stride;
+        const unsigned over = ~__ballot_sync(0xffffffffu, at < end && begins(at, key));
+        const int n = over ? __ffs(over) - 1 : 32;
+        const long long next = last + (n + 1) * stride;
+        last += n * stride;
+        end = next < end ? next : end;
     }
-#pragma unroll
-    for (int j = 0; j < Q; ++j) sum[j] = 0.f;
+    if (last - k0 <= JOIN_SHORT) return;  // a short one
+    Vals<Q> sum = splat<Q>(0.f);
     if (c < a.D) {
-#pragma unroll 4
-        for (long long k = k0 + down; k <= last; k += JOIN_DOWN) {
-            const Pack<float, Q> h = *reinterpret_cast<const Pack<float, Q>*>(a.part + (k * 2 + (k == k0)) * a.D + c);
-#pragma unroll
-            for (int j = 0; j < Q; ++j) sum[j] += h.v[j];
-        }
+#pragma unroll 8
+        for (long long k = k0 + down; k <= last; k += JOIN_DOWN)
+            sum = add(sum, to_vals<float, Q>(*reinterpret_cast<const Pack<float, Q>*>(a.part + (k * 2 + (k == k0)) * a.D + c)));
     }
-#pragma unroll
-    for (int j = 0; j < Q; ++j) s_sum[down][across * Q + j] = sum[j];
+    s_sum[down][lane] = to_pack<float, Q>(sum);
     __syncthreads();
     if (down || c >= a.D) return;
-    for (int d = 1; d < JOIN_DOWN; ++d) {
-#pragma unroll
-        for (int j = 0; j < Q; ++j) sum[j] += s_sum[d][across * Q + j];
-    }
+    for (int d = 1; d < JOIN_DOWN; ++d) sum = add(sum, to_vals<float, Q>(s_sum[d][lane]));
     store_row<T, Q>(d_table + (long long)key * a.D + c, sum, a.scale);
 }
 
@@ -516,18 +564,18 @@ struct EmbedPlan {
     size_t off_keys[2], off_places[2], off_hist, off_totals, off_count, off_part, bytes;
 };
 
-static int plan_embed_grad(long long n, long long rows, long long D, int device, EmbedPlan* p) {
+static int plan_embed_grad(long long n, long long rows, long long D, int dtype, int device, EmbedPlan* p) {
     if (n > EMBED_MAX_PLACES || rows > EMBED_MAX_ROWS || D > EMBED_MAX_WIDTH) return IGS_ERR_LIMIT;
     int bits = 1;
     while ((1ll << bits) < rows) ++bits;
     p->passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
     p->bits = (bits + p->passes - 1) / p->passes;
     p->n_blocks = (int)((n + SORT_BLOCK - 1) / SORT_BLOCK);
-    // enough chunks to fill the device with threads of one 16-byte pack each, none shorter than
-    // CHUNK_STEP places (packs of 4 values are counted: half as many threads do for 16-bit ones)
-    const long long threads_per_chunk = (D + 3) / 4;
-    long long chunks = (long long)sm_count(device) * 1024 / threads_per_chunk;
-    if (chunks < sm_count(device) / 4) chunks = sm_count(device) / 4;
+    // Chunks for 512 threads an SM with a 16-byte pack of columns each (fewer bytes a thread, where rows are
+    // no multiple of 16 bytes, only make more threads), none shorter than CHUNK_STEP places.
+    const long long threads_per_chunk = (D * (long long)dtype_size(dtype) + 15) / 16;
+    long long chunks = (long long)sm_count(device) * 512 / threads_per_chunk;
+    if (chunks < sm_count(device) / 2) chunks = sm_count(device) / 2;
     if (chunks > (n + CHUNK_STEP - 1) / CHUNK_STEP) chunks = (n + CHUNK_STEP - 1) / CHUNK_STEP;
     p->chunks = (int)(chunks < 1 ? 1 : chunks);
     size_t at = 0;
@@ -603,10 +651,11 @@ extern "C" int igs_embed(const void* tokens, int token_bytes, long long n, const
     return (int)cudaGetLastError();
 }
 
-extern "C" int igs_embed_grad_workspace_bytes(long long n, long long rows, long long D, int device, size_t* bytes) {
-    if (n < 0 || rows < 1 || D < 1 || !bytes) return IGS_ERR_ARG;
+extern "C" int igs_embed_grad_workspace_bytes(long long n, long long rows, long long D, int dtype, int device,
+                                              size_t* bytes) {
+    if (n < 0 || rows < 1 || D < 1 || !dtype_ok(dtype) || !bytes) return IGS_ERR_ARG;
     EmbedPlan p;
-    const int rc = plan_embed_grad(n, rows, D, device, &p);
+    const int rc = plan_embed_grad(n, rows, D, dtype, device, &p);
     if (rc) return rc;
     *bytes = p.bytes;
     return IGS_OK;
@@ -619,7 +668,7 @@ extern "C" int igs_embed_grad(const void* tokens, int token_bytes, long long n, 
     if (rc) return rc;
     if (!d_table || (n > 0 && (!tokens || !dy))) return IGS_ERR_ARG;
     EmbedPlan p;
-    rc = plan_embed_grad(n, rows, D, device, &p);
+    rc = plan_embed_grad(n, rows, D, dtype, device, &p);
     if (rc) return rc;
     if (n > 0 && (!workspace || workspace_bytes < p.bytes || !aligned_to(workspace, 16))) return IGS_ERR_WORKSPACE;
     DeviceGuard guard(device);
@@ -672,10 +721,10 @@ extern "C" int igs_embed_grad(const void* tokens, int token_bytes, long long n, 
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         if (packed) {
-            segment_kernel<T, 16 / sizeof(T)><<<grid, EMBED_THREADS, 0, s>>>(a);
+            segment_kernel<T, 16 / sizeof(T)><<<grid, EMBED_THREADS, segment_smem<T, 16 / sizeof(T)>, s>>>(a);
             if (joins) join_kernel<T, 4><<<joins, JOIN_THREADS, 0, s>>>(a, (int)short_blocks, (int)short_slabs);
         } else {
-            segment_kernel<T, 1><<<grid, EMBED_THREADS, 0, s>>>(a);
+            segment_kernel<T, 1><<<grid, EMBED_THREADS, segment_smem<T, 1>, s>>>(a);
             if (joins) join_kernel<T, 1><<<joins, JOIN_THREADS, 0, s>>>(a, (int)short_blocks, (int)short_slabs);
         }
         return 0;

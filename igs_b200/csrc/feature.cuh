@@ -163,6 +163,22 @@ __host__ __device__ inline bool aligned_to(const void* p, size_t bytes) {
     return reinterpret_cast<uintptr_t>(p) % bytes == 0;
 }
 
+// Asynchronous copies to shared memory, by which a thread reads ahead of itself: BYTES of 4 or 16, groups in
+// order of their commits.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);

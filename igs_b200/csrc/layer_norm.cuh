@@ -144,20 +144,6 @@ inline int norm_pack_bytes(const void* x, const void* y, const void* z, const vo
     return (int)tsize;
 }
 
-// What a thread copies ahead: PACK bytes of 4 or 16.
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src) {
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
-}
-
 // 16-bit values one by one cannot be copied that way.
 template <typename T, int V>
 constexpr bool norm_async = sizeof(Pack<T, V>) >= 4;

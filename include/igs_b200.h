@@ -420,7 +420,8 @@ int igs_embed(const void* tokens, int token_bytes, long long n, const void* tabl
  * The workspace starts on a 16-byte boundary.
  * No floating-point atomics: the same bits on every call.
  */
-int igs_embed_grad_workspace_bytes(long long n, long long rows, long long D, int device, size_t* bytes);
+int igs_embed_grad_workspace_bytes(long long n, long long rows, long long D, int dtype, int device,
+                                   size_t* bytes);
 int igs_embed_grad(const void* tokens, int token_bytes, long long n, const void* dy, int dtype,
                    long long rows, long long D, float scale, int has_empty, long long empty,
                    void* d_table, void* workspace, size_t workspace_bytes, int device, void* stream);

@@ -39,9 +39,9 @@ def test_c_abi_refuses_bad_arguments_before_any_cuda_call():
     assert embed(n=0, tok=None, out=None) == 0
 
     size = ctypes.c_size_t(0)
-    assert lib.igs_embed_grad_workspace_bytes(4, 5, 8, 0, None) == -1
-    assert lib.igs_embed_grad_workspace_bytes(4, 0, 8, 0, ctypes.byref(size)) == -1
-    assert lib.igs_embed_grad_workspace_bytes(1 << 31, 5, 8, 0, ctypes.byref(size)) == -3
+    assert lib.igs_embed_grad_workspace_bytes(4, 5, 8, 0, 0, None) == -1
+    assert lib.igs_embed_grad_workspace_bytes(4, 0, 8, 0, 0, ctypes.byref(size)) == -1
+    assert lib.igs_embed_grad_workspace_bytes(1 << 31, 5, 8, 0, 0, ctypes.byref(size)) == -3
 
     def embed_grad(tok=one, n=4, dy=one, dt=0, rows=5, D=8, scale=1.0, out=one, ws=one, nb=1 << 30):
         return lib.igs_embed_grad(tok, 8, n, dy, dt, rows, D, scale, 0, 0, out, ws, nb, 0, None)
