@@ -49,6 +49,24 @@ __device__ __forceinline__ uint32_t row_of(const Tokens& t, long long tok) {
     return tok >= 0 && tok < t.rows ? (uint32_t)tok : NO_ROW;
 }
 
+// The pack sizes in bytes that the kernels move, the widest on whose boundary all rows start.
+static int embed_pack_bytes(const void* a, const void* b, long long D, long long row_stride, size_t size) {
+    for (size_t bytes : {size_t(16), size_t(4)})
+        if (bytes > size && aligned_to(a, bytes) && aligned_to(b, bytes) && (size_t)D * size % bytes == 0 &&
+            (size_t)row_stride * size % bytes == 0)
+            return (int)bytes;
+    return (int)size;
+}
+
+// log2 of the threads that share a row of `packs` packs: the narrowest power of two that covers
+// it, a whole block at most
+static int group_log(long long packs) {
+    int g = 0;
+    while (g < 7 && (1 << g) < packs) ++g;
+    static_assert(EMBED_THREADS == 1 << 7, "a block is the widest group");
+    return g;
+}
+
 // ---------------------------------------------------------------------------
 // lookup
 // ---------------------------------------------------------------------------
@@ -60,11 +78,11 @@ struct EmbedArgs {
     float scale;
 };
 
-// A group of 2^log_g threads copies R rows, packs of V values a thread: the R tokens, then R
-// independent loads in flight per pack.
-template <typename T, int V, int R>
+// A group of 2^log_g threads copies R rows, U packs of V values a thread at a time: the R tokens, then
+// R U independent loads in flight.
+template <typename T, int V, int R, int U>
 __global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(EmbedArgs a, int log_g) {
-    const int lane = threadIdx.x & ((1 << log_g) - 1);
+    const int g = 1 << log_g, lane = threadIdx.x & (g - 1);
     const long long i0 = ((long long)blockIdx.x * (EMBED_THREADS >> log_g) + (threadIdx.x >> log_g)) * R;
     uint32_t row[R];
     float none[R];  // what fills the row of a place without one
@@ -79,20 +97,44 @@ __global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(EmbedArgs a, int l
             if (!(a.tokens.has_empty && tok == a.tokens.empty)) none[r] = __int_as_float(0x7fc00000);
         }
     }
-    const long long packs = a.D / V;
-    for (long long p = lane; p < packs; p += 1 << log_g) {
-        Pack<T, V> v[R];
+    const int packs = (int)(a.D / V);
+    for (int p0 = lane; p0 < packs; p0 += g * U) {
+        Pack<T, V> v[R][U];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (row[r] != NO_ROW)
-                v[r] = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.table) + (long long)row[r] * a.row_stride)[p];
+        for (int r = 0; r < R; ++r) {
+            const Pack<T, V>* src = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.table) + (long long)row[r] * a.row_stride);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (row[r] != NO_ROW && p0 + u * g < packs) v[r][u] = src[p0 + u * g];
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if (i0 + r >= a.n) continue;
-            const Vals<V> y = row[r] != NO_ROW ? mul(to_vals<T, V>(v[r]), splat<V>(a.scale)) : splat<V>(none[r]);
-            reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.out) + (i0 + r) * a.D)[p] = to_pack<T, V>(y);
+            Pack<T, V>* out = reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.out) + (i0 + r) * a.D);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (p0 + u * g >= packs) continue;
+                const Vals<V> y = row[r] != NO_ROW ? mul(to_vals<T, V>(v[r][u]), splat<V>(a.scale)) : splat<V>(none[r]);
+                out[p0 + u * g] = to_pack<T, V>(y);
+            }
         }
     }
+}
+
+template <typename T, int V>
+static void launch_embed(const EmbedArgs& a, int device, cudaStream_t s) {
+    // Four loads in flight a thread (with two or eight 65536 rows of 1024 bf16 took 37 and 43 us instead of
+    // 35): over rows where a row has one pack a thread, within the row where it has more.  Rows go
+    // several to a group once that still leaves every SM sixteen blocks; below, latency counts.
+    constexpr int MOST = 4;
+    const int log_g = group_log(a.D / V);
+    const long long groups = EMBED_THREADS >> log_g;
+    const bool wide = a.D / V > EMBED_THREADS, many = a.n >= (long long)sm_count(device) * 16 * groups * MOST;
+    const long long per = groups * (many && !wide ? MOST : 1);
+    const unsigned grid = (unsigned)((a.n + per - 1) / per);
+    if (wide) embed_kernel<T, V, 1, MOST><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
+    else if (many) embed_kernel<T, V, MOST, 1><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
+    else embed_kernel<T, V, 1, 1><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
 }
 
 // ---------------------------------------------------------------------------
@@ -135,13 +177,24 @@ __global__ void __launch_bounds__(RANK_WARPS * 32) sort_rank_kernel(SortArgs a) 
     __shared__ __align__(16) uint32_t s_key[RANK_MAX];
     __shared__ int s_rank[RANK_WARPS][32];
     __shared__ int s_held[RANK_WARPS];
+    let_next_start();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int n = (int)a.n, padded = (n + 31) / 32 * 32;
     int held = 0;
-    for (int i = threadIdx.x; i < padded; i += RANK_WARPS * 32) {
-        const uint32_t k = i < n ? row_of(a.tokens, token_at(a.tokens, i)) : NO_ROW;
-        s_key[i] = k;
-        held += k != NO_ROW;
+    for (int i0 = 0; i0 < padded; i0 += RANK_WARPS * 32 * 8) {  // (eight loads on their way together)
+        long long tok[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j * (RANK_WARPS * 32) + threadIdx.x;
+            if (i < n) tok[j] = token_at(a.tokens, i);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j * (RANK_WARPS * 32) + threadIdx.x;
+            const uint32_t k = i < n ? row_of(a.tokens, tok[j]) : NO_ROW;
+            if (i < padded) s_key[i] = k;
+            held += k != NO_ROW;
+        }
     }
     __syncthreads();
     const int mine = blockIdx.x * 32 + lane;
@@ -185,8 +238,10 @@ __global__ void __launch_bounds__(RANK_WARPS * 32) sort_rank_kernel(SortArgs a) 
 
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(SortArgs a) {
     __shared__ int s_hist[SORT_MAX_DIGITS];
+    let_next_start();
     for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) s_hist[d] = 0;
     __syncthreads();
+    if (a.keys_in) wait_for_previous();  // (the first pass reads tokens only; what it writes, nothing before it reads)
     const long long count = a.keys_in ? *a.count_in : a.n;
     const long long base = (long long)blockIdx.x * SORT_BLOCK;
     uint32_t key[SORT_BLOCK / SORT_THREADS];
@@ -206,6 +261,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(SortArgs a) {
 
 // a warp per digit: exclusive prefix sums over the blocks, and the digit's total
 __global__ void __launch_bounds__(SORT_THREADS) sort_scan_kernel(SortArgs a) {
+    let_next_start();
+    wait_for_previous();
     const int d = blockIdx.x * SORT_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (d >= a.digits) return;
     int* h = a.hist + (long long)d * a.n_blocks;
@@ -232,6 +289,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(SortArgs a) {
     __shared__ int s_sum[SORT_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
+    let_next_start();
+    if (a.keys_in) wait_for_previous();  // (the first pass reads tokens before)
     const long long count = a.keys_in ? *a.count_in : a.n;
     const long long base = (long long)blockIdx.x * SORT_BLOCK + (long long)warp * SORT_PER_WARP;
     uint32_t key[SORT_PER_WARP / 32];
@@ -240,13 +299,16 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(SortArgs a) {
     for (int j = 0; j < SORT_PER_WARP / 32; ++j)
         if (!sort_load(a, base + j * 32 + lane, count, key[j], place[j])) key[j] = NO_ROW;
 
+    if (!a.keys_in) wait_for_previous();
+
     // first slot of every digit: exclusive sums of the totals, four digits a thread
     constexpr int PER = SORT_MAX_DIGITS / SORT_THREADS;
-    int t[PER], sum = 0;
+    int t[PER], h[PER], sum = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int d = threadIdx.x * PER + j;
         t[j] = d < a.digits ? a.totals[d] : 0;
+        h[j] = d < a.digits ? a.hist[(long long)d * a.n_blocks + blockIdx.x] : 0;
         sum += t[j];
     }
     int incl = sum;
@@ -263,7 +325,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(SortArgs a) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int d = threadIdx.x * PER + j;
-        if (d < a.digits) s_first[d] = run + a.hist[(long long)d * a.n_blocks + blockIdx.x];
+        if (d < a.digits) s_first[d] = run + h[j];
         run += t[j];
     }
     if (a.count_out && blockIdx.x == 0 && threadIdx.x == SORT_THREADS - 1) *a.count_out = run;
@@ -318,7 +380,7 @@ struct SegmentArgs {
     float scale;
     int chunks;
     int sum_blocks;         // blocks of the segment kernel that sum; the others write zero rows
-    int log_g;              // a chunk is summed by 2^log_g threads, a pack of columns each
+    int log_g;              // a chunk is summed by 2^log_g threads a slab of columns
 };
 
 constexpr int CHUNK_STEP = 8;  // places whose rows are loaded together; chunks are multiples of it
@@ -327,8 +389,12 @@ constexpr int CHUNK_STEP = 8;  // places whose rows are loaded together; chunks 
 constexpr int SEGMENT_STAGES = 3;
 template <typename T, int V>
 constexpr bool segment_async = sizeof(Pack<T, V>) >= 4;
+// Packs of columns a thread: one of 16 bytes, or four small ones (a group's width apart).
 template <typename T, int V>
-constexpr size_t segment_smem = segment_async<T, V> ? sizeof(Pack<T, V>) * CHUNK_STEP * SEGMENT_STAGES * EMBED_THREADS : 0;
+constexpr int segment_items = sizeof(Pack<T, V>) == 16 ? 1 : 4;
+template <typename T, int V>
+constexpr size_t segment_smem =
+    segment_async<T, V> ? sizeof(Pack<T, V>) * segment_items<T, V> * CHUNK_STEP * SEGMENT_STAGES * EMBED_THREADS : 0;
 
 // positions a chunk holds, the last one's less
 __device__ __forceinline__ long long chunk_length(long long count, int chunks) {
@@ -345,34 +411,29 @@ __device__ __forceinline__ bool has_key(const uint32_t* keys, int count, uint32_
     return lo < count && keys[lo] == row;
 }
 
-// sum * scale to a row of the table
+// sum * scale to a pack of a row of the table
 template <typename T, int V>
-__device__ __forceinline__ void store_row(T* row, const Vals<V>& sum, float scale) {
-    *reinterpret_cast<Pack<T, V>*>(row) = to_pack<T, V>(mul(sum, splat<V>(scale)));
-}
-template <int V>
-__device__ __forceinline__ void store_part(float* part, const Vals<V>& sum) {
-    *reinterpret_cast<Pack<float, V>*>(part) = to_pack<float, V>(sum);
+__device__ __forceinline__ void store_pack(T* row, long long pack, const Vals<V>& sum, float scale) {
+    reinterpret_cast<Pack<T, V>*>(row)[pack] = to_pack<T, V>(mul(sum, splat<V>(scale)));
 }
 
-// grid (sum blocks + zero blocks, column slabs).  Every thread owns one pack of V columns and copies the
+// grid (sum blocks + zero blocks, column slabs).  Every thread owns its packs of V columns and copies the
 // rows of the next steps to shared memory of its own ahead of time: rows lie anywhere in dy, and what
 // bounds the kernel is how many of them are on their way (plain loads, eight a thread between
-// additions: 85 us for 65536 rows of 1024 bf16; the ring: NEWTIME).
+// additions: 85 us for 65536 rows of 1024 bf16; the ring: 35).
 template <typename T, int V>
 __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
-    const int count = *a.count;
+    constexpr int ITEMS = segment_items<T, V>;
+    let_next_start();
+    wait_for_previous();
+    const int count = *a.count, g = 1 << a.log_g;
     T* d_table = static_cast<T*>(a.d_table);
-    const long long packs = a.D / V;
+    const int packs = (int)(a.D / V), first_pack = (int)blockIdx.y * g * ITEMS;
     if ((int)blockIdx.x >= a.sum_blocks) {
         // rows without a token: a warp looks up 32 rows at a time, then writes those that have none
-        const int lane = threadIdx.x & 31;
-        const long long first = (long long)blockIdx.y << a.log_g;
-        const long long last = first + (1ll << a.log_g) < packs ? first + (1ll << a.log_g) : packs;
+        const int lane = threadIdx.x & 31, last_pack = first_pack + g * ITEMS < packs ? first_pack + g * ITEMS : packs;
         const long long warps = (long long)(gridDim.x - a.sum_blocks) * (EMBED_THREADS / 32);
-        Pack<T, V> zero;
-#pragma unroll
-        for (int j = 0; j < V; ++j) zero.v[j] = from_f<T>(0.f);
+        const Pack<T, V> zero = to_pack<T, V>(splat<V>(0.f));
         for (long long r0 = ((long long)(blockIdx.x - a.sum_blocks) * (EMBED_THREADS / 32) + (threadIdx.x >> 5)) * 32;
              r0 < a.rows; r0 += warps * 32) {
             const long long r = r0 + lane;
@@ -381,24 +442,28 @@ __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
                 const int k = __ffs(absent) - 1;
                 absent &= absent - 1;
                 Pack<T, V>* row = reinterpret_cast<Pack<T, V>*>(d_table + (r0 + k) * a.D);
-                for (long long p = first + lane; p < last; p += 32) row[p] = zero;
+                for (int p = first_pack + lane; p < last_pack; p += 32) row[p] = zero;
             }
         }
         return;
     }
     const long long chunk = (long long)blockIdx.x * (EMBED_THREADS >> a.log_g) + (threadIdx.x >> a.log_g);
-    const long long pack = ((long long)blockIdx.y << a.log_g) + (threadIdx.x & ((1 << a.log_g) - 1));
+    const int pack = first_pack + (threadIdx.x & (g - 1)), mine = packs - pack;  // (item i is there when i g < mine)
     const long long len = chunk_length(count, a.chunks), lo = chunk * len;
     const long long hi = lo + len < count ? lo + len : count;
-    if (chunk >= a.chunks || pack >= packs || lo >= hi) return;
-    const T* dy = static_cast<const T*>(a.dy) + pack * V;
-    d_table += pack * V;
-    float* part = a.part + chunk * 2 * a.D + pack * V;
+    if (chunk >= a.chunks || mine <= 0 || lo >= hi) return;
+    const T* dy = static_cast<const T*>(a.dy) + (long long)pack * V;
+    d_table += (long long)pack * V;
+    float* part = a.part + chunk * 2 * a.D + (long long)pack * V;
     const bool from_before = lo > 0 && a.keys[lo - 1] == a.keys[lo];
     const bool goes_on = hi < count && a.keys[hi] == a.keys[hi - 1];
     constexpr bool ASYNC = segment_async<T, V>;
     extern __shared__ __align__(16) unsigned char s_mem[];
     Pack<T, V>* ring = reinterpret_cast<Pack<T, V>*>(s_mem) + threadIdx.x;
+    const auto slot = [&](int stage, int u, int i) { return ring + ((stage * CHUNK_STEP + u) * ITEMS + i) * EMBED_THREADS; };
+    const auto source = [&](int place, int i) {
+        return reinterpret_cast<const Pack<T, V>*>(dy + (long long)place * a.D) + i * g;
+    };
 
     // Keys and places of a step (lo is a multiple of CHUNK_STEP and the sort's arrays are padded to 256
     // bytes: whole packs; what lies behind hi is not used)
@@ -416,10 +481,12 @@ __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
     };
     const auto fetch = [&](long long p, const Step& s, int stage) {
 #pragma unroll
-        for (int u = 0; u < CHUNK_STEP; ++u)
-            if (p + u < hi)
-                copy_async<sizeof(Pack<T, V>)>(ring + (stage * CHUNK_STEP + u) * EMBED_THREADS,
-                                               dy + (long long)s.place[u / 4].v[u % 4] * a.D);
+        for (int u = 0; u < CHUNK_STEP; ++u) {
+            if (p + u >= hi) break;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (i == 0 || i * g < mine) copy_async<sizeof(Pack<T, V>)>(slot(stage, u, i), source(s.place[u / 4].v[u % 4], i));
+        }
     };
 
     // pipeline: step i is added while the rows of i + 1 and i + 2 are on their way and the places of
@@ -437,60 +504,75 @@ __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
     }
     uint32_t key = s0.key[0].v[0];
     bool first = true;
-    Vals<V> sum = splat<V>(0.f);
+    Vals<V> sum[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) sum[i] = splat<V>(0.f);
+    // the sum of the run that ends here: `crosses` when it goes on in the next chunk
+    const auto finish_run = [&](bool crosses) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if (i > 0 && i * g >= mine) break;
+            if (first && from_before) reinterpret_cast<Pack<float, V>*>(part)[i * g] = to_pack<float, V>(sum[i]);
+            else if (crosses) reinterpret_cast<Pack<float, V>*>(part + a.D)[i * g] = to_pack<float, V>(sum[i]);
+            else store_pack<T, V>(d_table + (long long)key * a.D, i * g, sum[i], a.scale);
+            sum[i] = splat<V>(0.f);
+        }
+        first = false;
+    };
     int stage = 0;
     for (long long p = lo; p < hi; p += CHUNK_STEP) {
         load_step(p + 3 * CHUNK_STEP, s3);
-        Pack<T, V> v[CHUNK_STEP];
+        Pack<T, V> v[CHUNK_STEP][ITEMS];
         if constexpr (ASYNC) {
             fetch(p + 2 * CHUNK_STEP, s2, stage == 0 ? 2 : stage - 1);
             copy_commit();
             copy_wait<SEGMENT_STAGES - 1>();
-#pragma unroll
-            for (int u = 0; u < CHUNK_STEP; ++u)
-                if (p + u < hi) v[u] = ring[(stage * CHUNK_STEP + u) * EMBED_THREADS];
-            stage = stage == 2 ? 0 : stage + 1;
-        } else {
-#pragma unroll
-            for (int u = 0; u < CHUNK_STEP; ++u)
-                if (p + u < hi) v[u] = *reinterpret_cast<const Pack<T, V>*>(dy + (long long)s0.place[u / 4].v[u % 4] * a.D);
         }
+#pragma unroll
+        for (int u = 0; u < CHUNK_STEP; ++u) {
+            if (p + u >= hi) break;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                if (i > 0 && i * g >= mine) break;
+                if constexpr (ASYNC) v[u][i] = *slot(stage, u, i);
+                else v[u][i] = *source(s0.place[u / 4].v[u % 4], i);
+            }
+        }
+        stage = stage == 2 ? 0 : stage + 1;
 #pragma unroll
         for (int u = 0; u < CHUNK_STEP; ++u) {
             if (p + u >= hi) break;
             const uint32_t ku = s0.key[u / 4].v[u % 4];
             if (ku != key) {  // (the same in every thread of the group)
-                if (first && from_before) store_part<V>(part, sum);
-                else store_row<T, V>(d_table + (long long)key * a.D, sum, a.scale);
-                first = false;
+                finish_run(false);
                 key = ku;
-                sum = splat<V>(0.f);
             }
-            sum = add(sum, to_vals<T, V>(v[u]));
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (i == 0 || i * g < mine) sum[i] = add(sum[i], to_vals<T, V>(v[u][i]));
         }
         s0 = s1;
         s1 = s2;
         s2 = s3;
     }
     if constexpr (ASYNC) copy_wait<0>();
-    if (first && from_before) store_part<V>(part, sum);
-    else if (goes_on) store_part<V>(part + a.D, sum);
-    else store_row<T, V>(d_table + (long long)key * a.D, sum, a.scale);
+    finish_run(goes_on);
 }
 
 // Runs that cross chunk borders: the tail of the chunk in which the run starts, then the heads of
-// the chunks that follow.  Q columns (4, or 1 where D is odd) a thread.
-//   Short runs, up to JOIN_SHORT heads: the first `chunks` blocks of a slab, one per chunk that may
-//   start one; a thread adds its columns up.
+// the chunks that follow.  Q columns a thread.
+//   Short runs, up to JOIN_SHORT heads: in the first blocks `span` threads (whole warps) per chunk that
+//   may start one and slab of columns; a thread adds its columns up.
 //   Longer ones (they contain a chunk whose number is a multiple of JOIN_SHORT): one block per such
 //   chunk, which acts if it is the run's first.  32 threads across, 8 down: each of the 8 adds every
 //   8th row, and the 8 sums are added in order.
 constexpr int JOIN_SHORT = 16;
-constexpr int JOIN_THREADS = 256;
+constexpr int JOIN_THREADS = 512;
 constexpr int JOIN_DOWN = JOIN_THREADS / 32;
 template <typename T, int Q>
-__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(SegmentArgs a, int short_blocks, int short_slabs) {
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(SegmentArgs a, int short_blocks, int short_slabs, int span) {
     __shared__ Pack<float, Q> s_sum[JOIN_DOWN][32];
+    wait_for_previous();
     const int count = *a.count;
     const long long len = chunk_length(count, a.chunks);
     // whether chunk k exists and begins with the key / in the middle of a run of it
@@ -503,9 +585,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(SegmentArgs a, int s
     };
 
     if ((int)blockIdx.x < short_blocks) {
-        const long long k0 = blockIdx.x / short_slabs;
-        const long long c = ((long long)(blockIdx.x % short_slabs) * JOIN_THREADS + threadIdx.x) * Q;
-        if ((k0 + 1) * len >= count) return;
+        const long long unit = (long long)blockIdx.x * (JOIN_THREADS / span) + threadIdx.x / span;
+        const long long k0 = unit / short_slabs;
+        const long long c = ((unit % short_slabs) * span + threadIdx.x % span) * Q;
+        if ((k0 + 1) * len >= count) return;  // (the same in a whole warp, like what follows)
         const uint32_t key = a.keys[(k0 + 1) * len];
         // lane i looks at chunk k0 + 1 + i: how many chunks in a row begin with the key
         static_assert(JOIN_SHORT < 32, "a warp looks past a short run");
@@ -516,7 +599,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(SegmentArgs a, int s
         Vals<Q> sum = to_vals<float, Q>(*reinterpret_cast<const Pack<float, Q>*>(a.part + (k0 * 2 + 1) * a.D + c));
 #pragma unroll 4
         for (int i = 0; i < heads; ++i) sum = add(sum, head(k0 + 1 + i, c));
-        store_row<T, Q>(d_table + (long long)key * a.D + c, sum, a.scale);
+        store_pack<T, Q>(d_table + (long long)key * a.D + c, 0, sum, a.scale);
         return;
     }
 
@@ -553,7 +636,30 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(SegmentArgs a, int s
     __syncthreads();
     if (down || c >= a.D) return;
     for (int d = 1; d < JOIN_DOWN; ++d) sum = add(sum, to_vals<float, Q>(s_sum[d][lane]));
-    store_row<T, Q>(d_table + (long long)key * a.D + c, sum, a.scale);
+    store_pack<T, Q>(d_table + (long long)key * a.D + c, 0, sum, a.scale);
+}
+
+template <typename T, int V>
+static void launch_sums(SegmentArgs& a, cudaStream_t s) {
+    constexpr int Q = V < 4 ? V : 4;
+    const long long packs = a.D / V;
+    a.log_g = group_log((packs + segment_items<T, V> - 1) / segment_items<T, V>);
+    const int groups = EMBED_THREADS >> a.log_g, slab = segment_items<T, V> << a.log_g;
+    a.sum_blocks = (a.chunks + groups - 1) / groups;
+    const long long zero = (a.rows + EMBED_THREADS - 1) / EMBED_THREADS;
+    const dim3 grid((unsigned)(a.sum_blocks + (zero < 4096 ? zero : 4096)),
+                    (unsigned)((packs + slab - 1) / slab));
+    launch_chained(segment_kernel<T, V>, grid, EMBED_THREADS, segment_smem<T, V>, s, a);
+    count_launch();
+    int span = 32;
+    while (span < JOIN_THREADS && span * Q < a.D) span *= 2;
+    const long long short_slabs = (a.D + span * Q - 1) / (span * Q), long_slabs = (a.D + 32 * Q - 1) / (32 * Q);
+    const long long short_blocks = ((a.chunks - 1) * short_slabs * span + JOIN_THREADS - 1) / JOIN_THREADS;
+    const long long long_blocks = (a.chunks - 1) / JOIN_SHORT * long_slabs;
+    if (a.chunks == 1) return;
+    launch_chained(join_kernel<T, Q>, (unsigned)(short_blocks + long_blocks), JOIN_THREADS, 0, s, a, (int)short_blocks,
+                   (int)short_slabs, span);
+    count_launch();
 }
 
 // ---------------------------------------------------------------------------
@@ -571,10 +677,9 @@ static int plan_embed_grad(long long n, long long rows, long long D, int dtype, 
     p->passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
     p->bits = (bits + p->passes - 1) / p->passes;
     p->n_blocks = (int)((n + SORT_BLOCK - 1) / SORT_BLOCK);
-    // Chunks for 512 threads an SM with a 16-byte pack of columns each (fewer bytes a thread, where rows are
-    // no multiple of 16 bytes, only make more threads), none shorter than CHUNK_STEP places.
-    const long long threads_per_chunk = (D * (long long)dtype_size(dtype) + 15) / 16;
-    long long chunks = (long long)sm_count(device) * 512 / threads_per_chunk;
+    // One wave of blocks: 512 threads an SM, 16 bytes of columns a thread.
+    const long long packs = (D * (long long)dtype_size(dtype) + 15) / 16, g = 1ll << group_log(packs);
+    long long chunks = (long long)sm_count(device) * 512 / ((packs + g - 1) / g * g);
     if (chunks < sm_count(device) / 2) chunks = sm_count(device) / 2;
     if (chunks > (n + CHUNK_STEP - 1) / CHUNK_STEP) chunks = (n + CHUNK_STEP - 1) / CHUNK_STEP;
     p->chunks = (int)(chunks < 1 ? 1 : chunks);
@@ -594,15 +699,6 @@ static int plan_embed_grad(long long n, long long rows, long long D, int dtype, 
     p->off_part = take((size_t)p->chunks * 2 * D * 4);
     p->bytes = at;
     return IGS_OK;
-}
-
-// log2 of the threads that share a row of `packs` packs: the narrowest power of two that covers
-// it, a whole block at most
-static int group_log(long long packs) {
-    int g = 0;
-    while (g < 7 && (1 << g) < packs) ++g;
-    static_assert(EMBED_THREADS == 1 << 7, "a block is the widest group");
-    return g;
 }
 
 static int token_args_ok(int token_bytes, long long n, long long rows, long long D, int dtype, float scale) {
@@ -628,23 +724,12 @@ extern "C" int igs_embed(const void* tokens, int token_bytes, long long n, const
     if (!guard.ok) return IGS_ERR_DEVICE;
     cudaStream_t s = (cudaStream_t)stream;
     EmbedArgs a{{tokens, token_bytes == 8, has_empty != 0, empty, rows}, table, out, n, D, row_stride, scale};
-    const size_t size = dtype_size(dtype);
-    const bool packed = aligned_to(table, 16) && aligned_to(out, 16) && (size_t)D * size % 16 == 0 &&
-                        (size_t)row_stride * size % 16 == 0;
-    const long long packs = packed ? D * (long long)size / 16 : D;
-    const int log_g = group_log(packs);
-    // four rows a group once that still leaves every SM sixteen blocks; below, latency counts
-    const long long groups = EMBED_THREADS >> log_g;
-    const bool four = n >= (long long)sm_count(device) * 16 * groups * 4;
-    const long long per = groups * (four ? 4 : 1);
-    const unsigned grid = (unsigned)((n + per - 1) / per);
+    const int bytes = embed_pack_bytes(table, out, D, row_stride, dtype_size(dtype));
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        constexpr int V = 16 / sizeof(T);
-        if (packed && four) embed_kernel<T, V, 4><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
-        else if (packed) embed_kernel<T, V, 1><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
-        else if (four) embed_kernel<T, 1, 4><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
-        else embed_kernel<T, 1, 1><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
+        if (bytes == 16) launch_embed<T, 16 / sizeof(T)>(a, device, s);
+        else if (bytes == 4) launch_embed<T, 4 / sizeof(T)>(a, device, s);
+        else launch_embed<T, 1>(a, device, s);
         return 0;
     });
     count_launch();
@@ -702,33 +787,21 @@ extern "C" int igs_embed_grad(const void* tokens, int token_bytes, long long n, 
         so.places_out = reinterpret_cast<int*>(ws + p.off_places[to]);
         so.count_out = pass ? nullptr : count;
         so.shift = pass * p.bits;
-        sort_count_kernel<<<p.n_blocks, SORT_THREADS, 0, s>>>(so);
-        sort_scan_kernel<<<(so.digits + SORT_WARPS - 1) / SORT_WARPS, SORT_THREADS, 0, s>>>(so);
-        sort_place_kernel<<<p.n_blocks, SORT_THREADS, 0, s>>>(so);
+        if (!pass) sort_count_kernel<<<p.n_blocks, SORT_THREADS, 0, s>>>(so);
+        else launch_chained(sort_count_kernel, p.n_blocks, SORT_THREADS, 0, s, so);
+        launch_chained(sort_scan_kernel, (so.digits + SORT_WARPS - 1) / SORT_WARPS, SORT_THREADS, 0, s, so);
+        launch_chained(sort_place_kernel, p.n_blocks, SORT_THREADS, 0, s, so);
         count_launch(3);
     }
-    const bool packed = aligned_to(dy, 16) && aligned_to(d_table, 16) && (size_t)D * dtype_size(dtype) % 16 == 0;
-    const long long packs = packed ? D * (long long)dtype_size(dtype) / 16 : D;
-    const int log_g = group_log(packs), groups = EMBED_THREADS >> log_g;
     SegmentArgs a{so.keys_out, so.places_out, count, dy, d_table, reinterpret_cast<float*>(ws + p.off_part), rows, D,
-                  scale, p.chunks, (p.chunks + groups - 1) / groups, log_g};
-    const long long zero = (rows + EMBED_THREADS - 1) / EMBED_THREADS;
-    const dim3 grid((unsigned)(a.sum_blocks + (zero < 4096 ? zero : 4096)), (unsigned)((packs + (1 << log_g) - 1) >> log_g));
-    const long long q = packed ? 4 : 1;
-    const long long short_slabs = (D + JOIN_THREADS * q - 1) / (JOIN_THREADS * q), long_slabs = (D + 32 * q - 1) / (32 * q);
-    const long long short_blocks = (p.chunks - 1) * short_slabs, long_blocks = (p.chunks - 1) / JOIN_SHORT * long_slabs;
-    const unsigned joins = (unsigned)(short_blocks + long_blocks);
+                  scale, p.chunks, 0, 0};
+    const int bytes = embed_pack_bytes(dy, d_table, D, D, dtype_size(dtype));
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        if (packed) {
-            segment_kernel<T, 16 / sizeof(T)><<<grid, EMBED_THREADS, segment_smem<T, 16 / sizeof(T)>, s>>>(a);
-            if (joins) join_kernel<T, 4><<<joins, JOIN_THREADS, 0, s>>>(a, (int)short_blocks, (int)short_slabs);
-        } else {
-            segment_kernel<T, 1><<<grid, EMBED_THREADS, segment_smem<T, 1>, s>>>(a);
-            if (joins) join_kernel<T, 1><<<joins, JOIN_THREADS, 0, s>>>(a, (int)short_blocks, (int)short_slabs);
-        }
+        if (bytes == 16) launch_sums<T, 16 / sizeof(T)>(a, s);
+        else if (bytes == 4) launch_sums<T, 4 / sizeof(T)>(a, s);
+        else launch_sums<T, 1>(a, s);
         return 0;
     });
-    count_launch(joins ? 2 : 1);
     return (int)cudaGetLastError();
 }

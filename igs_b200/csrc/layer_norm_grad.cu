@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
     constexpr int STAGES = norm_stages<T, V>(2 * ITEMS * R, BLOCK);
     extern __shared__ __align__(16) unsigned char s_mem[];
     __shared__ float s_red[G > 32 ? 2 * (G / 32) * 2 * R : 1];
+    let_next_start();
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float inv_d = 1.f / (float)a.D;
     const int packs = (int)(a.D / V), mine = packs - lane;  // (item k is there when k G < mine)
@@ -266,6 +267,7 @@ template <typename W>
 __global__ void __launch_bounds__(32 * LN_FINISH_ROWS) layer_norm_finish_kernel(NormGradArgs a) {
     __shared__ float s_sum[LN_FINISH_ROWS][32];
     const long long i = (long long)blockIdx.x * 32 + threadIdx.x;
+    wait_for_previous();
     float s = 0.f;
     if (i < 2 * a.D) {
 #pragma unroll 8
@@ -334,7 +336,7 @@ static void launch_norm_grad(NormGradArgs& a, int device, cudaStream_t s) {
         }
     }
     if (a.dw || a.db) {
-        layer_norm_finish_kernel<W><<<(unsigned)((2 * a.D + 31) / 32), dim3(32, LN_FINISH_ROWS), 0, s>>>(a);
+        launch_chained(layer_norm_finish_kernel<W>, (unsigned)((2 * a.D + 31) / 32), dim3(32, LN_FINISH_ROWS), 0, s, a);
         count_launch();
     }
 }
