@@ -35,7 +35,6 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
     constexpr int STAGES = norm_stages<T, V>(2 * ITEMS * R, BLOCK);
     extern __shared__ __align__(16) unsigned char s_mem[];
     __shared__ float s_red[G > 32 ? 2 * (G / 32) * 2 * R : 1];
-    let_next_start();
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float inv_d = 1.f / (float)a.D;
     const int packs = (int)(a.D / V), mine = packs - lane;  // (item k is there when k G < mine)
@@ -170,6 +169,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
     }
 
     if constexpr (ASYNC) copy_wait<0>();
+    let_next_start();
     if (!a.dw && !a.db) return;
     float* part = a.part + (long long)blockIdx.x * 2 * a.D;
     if constexpr (GROUPS > 1) {
