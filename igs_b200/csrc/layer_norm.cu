@@ -124,9 +124,16 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stre
     const char* firsts = static_cast<const char*>(a.x) + first * x_row;
     char* out = static_cast<char*>(a.y) + first * y_row + lane * PACK;
     const char* now = ahead;  // (used where nothing is copied ahead)
-    long long ahead_left = a.rows - first;
+    // A group makes `steps` steps, the last with `tail` rows (none or fewer, where narrow groups share a
+    // warp).  A warp goes on while it has a row; narrower groups share one and go on together, a wider
+    // group is the block: barriers and exchanges are met by all of their threads.
+    const long long ours = a.rows - (G == 32 ? first : first - group * R);
+    const int steps = ours > 0 ? (int)((ours + step - 1) / step) : 0;
+    const int tail = (int)(a.rows - first - (steps - 1) * step < R ? a.rows - first - (steps - 1) * step : R);
+    RowStats* stats = a.stats ? a.stats + first : nullptr;
+    int fetched = 0;
     const auto fetch = [&](int stage) {
-        const int n = (int)(ahead_left < R ? ahead_left : R);
+        const int n = fetched < steps - 1 ? R : fetched == steps - 1 ? tail : 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if (r >= n) break;
@@ -135,7 +142,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stre
                 if (k < FULL || k * G < mine) copy_async<PACK>(slot(stage, r, k), ahead + r * x_row + k * (G * PACK));
         }
         ahead += step * x_row;
-        ahead_left -= step;
+        ++fetched;
     };
     if constexpr (ASYNC) {
 #pragma unroll
@@ -148,22 +155,20 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stre
     stage_weights<W, V>(s_b, a.b, 0.f, (int)a.D, packs, BLOCK);
     // A row's first value: lane 0 holds it; in groups wider than a warp it is loaded one batch ahead.
     float next[R];
-    const auto fetch_first = [&](long long rows_left) {
+    const auto fetch_first = [&](int i) {
         if constexpr (G > 32) {
-            const int n = (int)(rows_left < R ? rows_left : R);
+            const int n = i < steps - 1 ? R : i == steps - 1 ? tail : 0;
 #pragma unroll
             for (int r = 0; r < R; ++r) next[r] = r < n ? to_f(*reinterpret_cast<const T*>(firsts + r * x_row)) : 0.f;
             firsts += step * x_row;
         }
     };
-    fetch_first(a.rows - first);
+    fetch_first(0);
     __syncthreads();
 
     int stage = 0;
-    // (a warp goes on while it has a row; narrower groups share one and go on together, a wider group
-    // is the block: barriers and exchanges are met by all of their threads)
-    for (long long row0 = first, base = G == 32 ? first : first - group * R; base < a.rows; row0 += step, base += step) {
-        const int left = (int)(a.rows - row0 < R ? a.rows - row0 : R);
+    for (int i = 0; i < steps; ++i) {
+        const int left = i < steps - 1 ? R : tail;
         Vals<V> d[R][ITEMS];
         float x0[R], shift[R], rstd[R];
         if constexpr (ASYNC) {
@@ -193,7 +198,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stre
             shift[r] = total(sum);
         }
         now += step * x_row;
-        fetch_first(a.rows - row0 - step);
+        fetch_first(i + 1);
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         group_sum<G, R>(shift, s_red, 0);
 #pragma unroll
@@ -212,8 +217,9 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stre
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             rstd[r] = rsqrtf(rstd[r] * inv_d + a.eps);
-            if (lane == 0 && a.stats && r < left) a.stats[row0 + r] = RowStats{x0[r], shift[r], rstd[r], 0.f};
+            if (lane == 0 && stats && r < left) stats[r] = RowStats{x0[r], shift[r], rstd[r], 0.f};
         }
+        if (stats) stats += step;
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {
             if (k >= FULL && k * G >= mine) continue;

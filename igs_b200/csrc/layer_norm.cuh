@@ -105,8 +105,8 @@ __device__ __forceinline__ Vals<V> staged_weights(const float* s_w, int pack, in
 // false when none does: up to 32 values a thread of 16-bit types, 16 of 32-bit ones (the same bytes in
 // flight a thread).  As few threads a row as possible, since what a row costs beside its values (two
 // sums across its threads, addresses, its statistics) is paid per thread.  The first FULL items are
-// there in every thread: a check per item costs registers and moves (all items checked, the gradient
-// of 65536 x 1024 bf16 took 88 us instead of 71).
+// there in every thread: a check per item costs registers and moves (the gradient of 65536 x 1024 bf16
+// takes 81 us without, 87 with the last of four items checked, 93 with all).
 template <int N>
 struct Int {
     static constexpr int value = N;
@@ -115,18 +115,25 @@ template <typename T, int V, typename F>
 inline bool with_stream_group(long long packs, F&& f) {
     constexpr int J = 16 / V, I = sizeof(T) == 2 && V > 1 ? 2 * J : J;  // the most packs a thread
     constexpr int Q = I / 4, H = I / 2;
-    if (packs <= 8) f(Int<8>{}, Int<1>{}, Int<0>{});
-    else if (packs <= 32) f(Int<32>{}, Int<1>{}, Int<0>{});
-    else if (Q > 1 && packs <= 32 * Q) f(Int<32>{}, Int<Q>{}, Int<1>{});
-    else if (packs <= 32 * H) f(Int<32>{}, Int<H>{}, Int<Q>{});
-    else if (packs <= 32 * (H + Q)) f(Int<32>{}, Int<H + Q>{}, Int<H>{});
-    else if (packs <= 32 * I) f(Int<32>{}, Int<I>{}, Int<H + Q>{});
-    else if (packs <= 64 * (H + Q)) f(Int<64>{}, Int<H + Q>{}, Int<H>{});
-    else if (packs <= 64 * I) f(Int<64>{}, Int<I>{}, Int<H + Q>{});
-    else if (packs <= 128 * (H + Q)) f(Int<128>{}, Int<H + Q>{}, Int<H>{});
-    else if (packs <= 128 * I) f(Int<128>{}, Int<I>{}, Int<H + Q>{});
-    else if (I == J && packs <= 256 * J) f(Int<256>{}, Int<J>{}, Int<J / 2>{});
-    else if (packs <= 512 * J) f(Int<512>{}, Int<J>{}, Int<J / 2>{});
+    // (widths that fill their group to the last thread, as round ones do, have no check at all)
+    const auto go = [&](auto g, auto items, auto full) {
+        if constexpr (V * sizeof(T) == 16) {
+            if (packs == (long long)decltype(g)::value * decltype(items)::value) return f(g, items, items);
+        }
+        f(g, items, full);
+    };
+    if (packs <= 8) go(Int<8>{}, Int<1>{}, Int<0>{});
+    else if (packs <= 32) go(Int<32>{}, Int<1>{}, Int<0>{});
+    else if (Q > 1 && packs <= 32 * Q) go(Int<32>{}, Int<Q>{}, Int<1>{});
+    else if (packs <= 32 * H) go(Int<32>{}, Int<H>{}, Int<Q>{});
+    else if (packs <= 32 * (H + Q)) go(Int<32>{}, Int<H + Q>{}, Int<H>{});
+    else if (packs <= 32 * I) go(Int<32>{}, Int<I>{}, Int<H + Q>{});
+    else if (packs <= 64 * (H + Q)) go(Int<64>{}, Int<H + Q>{}, Int<H>{});
+    else if (packs <= 64 * I) go(Int<64>{}, Int<I>{}, Int<H + Q>{});
+    else if (packs <= 128 * (H + Q)) go(Int<128>{}, Int<H + Q>{}, Int<H>{});
+    else if (packs <= 128 * I) go(Int<128>{}, Int<I>{}, Int<H + Q>{});
+    else if (I == J && packs <= 256 * J) go(Int<256>{}, Int<J>{}, Int<J / 2>{});
+    else if (packs <= 512 * J) go(Int<512>{}, Int<J>{}, Int<J / 2>{});
     else return false;
     return true;
 }

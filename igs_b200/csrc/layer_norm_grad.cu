@@ -58,9 +58,15 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
     const char* dy_ahead = static_cast<const char*>(a.dy) + first * y_row + lane * PACK;
     const char *x_now = x_ahead, *dy_now = dy_ahead;  // (used where nothing is copied ahead)
     char* out = static_cast<char*>(a.dx) + first * y_row + lane * PACK;
-    long long ahead_left = a.rows - first;
+    // A group makes `steps` steps, the last with `tail` rows (none or fewer, where narrow groups share a
+    // warp).  A warp goes on while it has a row; narrower groups share one and go on together, a wider
+    // group is the block: barriers and exchanges are met by all of their threads.
+    const long long ours = a.rows - (G == 32 ? first : first - group * R);
+    const int steps = ours > 0 ? (int)((ours + step - 1) / step) : 0;
+    const int tail = (int)(a.rows - first - (steps - 1) * step < R ? a.rows - first - (steps - 1) * step : R);
+    int fetched = 0;
     const auto fetch = [&](int stage) {
-        const int n = (int)(ahead_left < R ? ahead_left : R);
+        const int n = fetched < steps - 1 ? R : fetched == steps - 1 ? tail : 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if (r >= n) break;
@@ -73,7 +79,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
         }
         x_ahead += step * x_row;
         dy_ahead += step * y_row;
-        ahead_left -= step;
+        ++fetched;
     };
     if constexpr (ASYNC) {
 #pragma unroll
@@ -85,21 +91,19 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
     // (a row's statistics are loaded one batch ahead; a row past the last has a factor of zero)
     RowStats next[R];
     const RowStats* stats = a.stats + first;
-    const auto fetch_stats = [&](long long rows_left) {
-        const int n = (int)(rows_left < R ? rows_left : R);
+    const auto fetch_stats = [&](int i) {
+        const int n = i < steps - 1 ? R : i == steps - 1 ? tail : 0;
 #pragma unroll
         for (int r = 0; r < R; ++r) next[r] = r < n ? stats[r] : RowStats{0.f, 0.f, 0.f, 0.f};
         stats += step;
     };
-    fetch_stats(a.rows - first);
+    fetch_stats(0);
     stage_weights<W, V>(s_w, a.w, 1.f, (int)a.D, packs, BLOCK);
     __syncthreads();
 
     int turn = 0, stage = 0;
-    // (a warp goes on while it has a row; narrower groups share one and go on together, a wider group
-    // is the block: barriers and exchanges are met by all of their threads)
-    for (long long row0 = first, base = G == 32 ? first : first - group * R; base < a.rows; row0 += step, base += step) {
-        const int left = (int)(a.rows - row0 < R ? a.rows - row0 : R);
+    for (int i = 0; i < steps; ++i) {
+        const int left = i < steps - 1 ? R : tail;
         Vals<V> xh[R][ITEMS], g[R][ITEMS];  // xhat and dy w
         float rstd[R], s[2 * R];
         if constexpr (ASYNC) {
@@ -147,7 +151,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
         }
         x_now += step * x_row;
         dy_now += step * y_row;
-        fetch_stats(a.rows - row0 - step);
+        fetch_stats(i + 1);
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         if (a.dx) {  // (the same for every thread)
             group_sum<G, 2 * R>(s, s_red, turn);
