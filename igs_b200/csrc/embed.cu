@@ -6,15 +6,16 @@
 // places of one token next to each other in their own order, so every row is one sum in 32 bits
 // with a fixed sequence and one rounding, the same bits on every run.
 //   1. sort.  Up to RANK_MAX places: one kernel ranks every place against all keys.  More: least
-//      significant digits first, up to 10 bits a pass (a codebook of a million rows needs two); per
-//      pass a count per block of places, a prefix sum over blocks, and the placement.  Places
-//      without a token in the table drop out.
+//      significant digits first, up to 10 bits a pass (a codebook of a million rows needs two).
+//      Places without a token in the table drop out.
 //   2. segments: the sorted places are cut into chunks of equal length whatever the tokens are
 //      (one common token may own most of them).  A run of one token inside a chunk is finished
 //      there; the sums of runs that cross a border go to the chunk's two partial rows ("head":
 //      it came from the chunk before, "tail": it started here and goes on).  The same launch
 //      writes the zero rows.
 //   3. join: the partial rows of a crossing run are added in order.
+#include <cooperative_groups.h>
+
 #include "feature.cuh"
 
 namespace igs {
@@ -142,30 +143,14 @@ static void launch_embed(const EmbedArgs& a, int device, cudaStream_t s) {
 // ---------------------------------------------------------------------------
 struct SortArgs {
     Tokens tokens;
-    const uint32_t* keys_in;   // NULL in the first pass: the tokens themselves
-    const int* places_in;
-    uint32_t* keys_out;
-    int* places_out;
-    int* hist;                 // [digits][blocks]: counts, then first slots within the digit
-    int* totals;               // [digits]
-    const int* count_in;       // how many (key, place) pairs the pass takes; first pass: n
-    int* count_out;            // first pass: how many places hold a token
+    uint32_t* keys[2];  // in and out of the passes in turn; the first pass reads the tokens
+    int* places[2];
+    int* hist;          // [digits][blocks]: how often each block meets a digit, then its first slot in the digit
+    int* totals;        // [digits]
+    int* count;         // how many places hold a token
     long long n;
-    int n_blocks, shift, digits;
+    int passes, bits;   // digits of `bits` bits
 };
-
-// the pair at position i of the pass's input; false when there is none
-__device__ __forceinline__ bool sort_load(const SortArgs& a, long long i, long long count, uint32_t& key, int& place) {
-    if (i >= count) return false;
-    if (a.keys_in) {
-        key = a.keys_in[i];
-        place = a.places_in[i];
-        return true;
-    }
-    key = row_of(a.tokens, token_at(a.tokens, i));
-    place = (int)i;
-    return key != NO_ROW;
-}
 
 // Few places: every place's slot is the number of keys below its own plus the number of equal ones
 // before it, counted over all keys.  Block b ranks the places 32 b .. 32 b + 31, one a lane; each
@@ -226,144 +211,161 @@ __global__ void __launch_bounds__(RANK_WARPS * 32) sort_rank_kernel(SortArgs a) 
 #pragma unroll
     for (int w = 0; w < RANK_WARPS; ++w) slot += s_rank[w][lane];
     if (mine < n && key != NO_ROW) {
-        a.keys_out[slot] = key;
-        a.places_out[slot] = mine;
+        a.keys[0][slot] = key;
+        a.places[0][slot] = mine;
     }
     if (blockIdx.x == 0 && lane == 0) {
         int sum = 0;
         for (int w = 0; w < RANK_WARPS; ++w) sum += s_held[w];
-        *a.count_out = sum;
+        *a.count = sum;
     }
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(SortArgs a) {
-    __shared__ int s_hist[SORT_MAX_DIGITS];
-    let_next_start();
-    for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) s_hist[d] = 0;
-    __syncthreads();
-    if (a.keys_in) wait_for_previous();  // (the first pass reads tokens only; what it writes, nothing before it reads)
-    const long long count = a.keys_in ? *a.count_in : a.n;
-    const long long base = (long long)blockIdx.x * SORT_BLOCK;
-    uint32_t key[SORT_BLOCK / SORT_THREADS];
-    bool ok[SORT_BLOCK / SORT_THREADS];
-#pragma unroll
-    for (int j = 0; j < SORT_BLOCK / SORT_THREADS; ++j) {
-        int place;
-        ok[j] = sort_load(a, base + j * SORT_THREADS + threadIdx.x, count, key[j], place);
-    }
-#pragma unroll
-    for (int j = 0; j < SORT_BLOCK / SORT_THREADS; ++j)
-        // (integer counts: the result does not depend on the order of the adds)
-        if (ok[j]) atomicAdd(&s_hist[(key[j] >> a.shift) & (a.digits - 1)], 1);
-    __syncthreads();
-    for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) a.hist[(long long)d * a.n_blocks + blockIdx.x] = s_hist[d];
-}
+// More places: all passes in one cooperative launch (three launches a pass took 19 us on the device for
+// 65536 places and two passes, this NEWTIME, and every launch costs the host 4).  Block b owns a range of
+// neighbouring positions.  A pass: it counts the digits of its range; once all have, it finds from the
+// counts where each digit of its range goes (behind all smaller digits, and behind the same digit of
+// the blocks before); then it ranks its range in order, 32 positions a warp at a time, and writes the pairs.
+__global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
+    __shared__ int s_first[SORT_MAX_DIGITS];             // counts, then the next slot per digit
+    __shared__ int s_warp[SORT_WARPS][SORT_MAX_DIGITS];  // per warp: counts, then first slots
+    __shared__ int s_sum[SORT_WARPS];
+    constexpr int PER = SORT_PER_WARP / 32;
+    const auto grid = cooperative_groups::this_grid();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = (int)gridDim.x;
+    const int digits = 1 << a.bits;
 
-// a warp per digit: exclusive prefix sums over the blocks, and the digit's total
-__global__ void __launch_bounds__(SORT_THREADS) sort_scan_kernel(SortArgs a) {
-    let_next_start();
-    wait_for_previous();
-    const int d = blockIdx.x * SORT_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (d >= a.digits) return;
-    int* h = a.hist + (long long)d * a.n_blocks;
-    int run = 0;
-    for (int b0 = 0; b0 < a.n_blocks; b0 += 32) {
-        const int b = b0 + lane;
-        const int v = b < a.n_blocks ? h[b] : 0;
-        int incl = v;
+    for (int pass = 0; pass < a.passes; ++pass) {
+        const uint32_t* keys_in = a.keys[(pass & 1) ^ 1];
+        const int* places_in = a.places[(pass & 1) ^ 1];
+        uint32_t* keys_out = a.keys[pass & 1];
+        int* places_out = a.places[pass & 1];
+        const int shift = pass * a.bits;
+        const long long count = pass ? *a.count : a.n;
+        const long long tiles = (count + SORT_BLOCK - 1) / SORT_BLOCK, each = (tiles + blocks - 1) / blocks;
+        const long long from = blockIdx.x * each * SORT_BLOCK;
+        const long long to = from + each * SORT_BLOCK < count ? from + each * SORT_BLOCK : count;
+        // position i of the pass's input; NO_ROW when there is none
+        const auto key_at = [&](long long i) {
+            if (i >= to) return NO_ROW;
+            return pass ? keys_in[i] : row_of(a.tokens, token_at(a.tokens, i));
+        };
+        const auto digit = [&](uint32_t key) { return (int)(key >> shift) & (digits - 1); };
+
+        for (int d = threadIdx.x; d < digits; d += SORT_THREADS) s_first[d] = 0;
+        __syncthreads();
+        for (long long t = from; t < to; t += SORT_BLOCK) {
+            uint32_t key[SORT_BLOCK / SORT_THREADS];
+#pragma unroll
+            for (int j = 0; j < SORT_BLOCK / SORT_THREADS; ++j) key[j] = key_at(t + j * SORT_THREADS + threadIdx.x);
+#pragma unroll
+            for (int j = 0; j < SORT_BLOCK / SORT_THREADS; ++j)
+                // (integer counts: the result does not depend on the order of the adds)
+                if (key[j] != NO_ROW) atomicAdd(&s_first[digit(key[j])], 1);
+        }
+        __syncthreads();
+        for (int d = threadIdx.x; d < digits; d += SORT_THREADS) a.hist[(long long)d * blocks + blockIdx.x] = s_first[d];
+        grid.sync();
+
+        // a warp per digit, dealt out over the blocks: exclusive sums over the blocks, and the total
+        for (int d = blockIdx.x + warp * blocks; d < digits; d += SORT_WARPS * blocks) {
+            int* h = a.hist + (long long)d * blocks;
+            int run = 0;
+            for (int b0 = 0; b0 < blocks; b0 += 32) {
+                const int b = b0 + lane, v = b < blocks ? h[b] : 0;
+                int incl = v;
+#pragma unroll
+                for (int s = 1; s < 32; s <<= 1) {
+                    const int t = __shfl_up_sync(0xffffffffu, incl, s);
+                    if (lane >= s) incl += t;
+                }
+                if (b < blocks) h[b] = run + incl - v;
+                run += __shfl_sync(0xffffffffu, incl, 31);
+            }
+            if (lane == 0) a.totals[d] = run;
+        }
+        grid.sync();
+
+        // first slots of this block's digits: exclusive sums of the totals, four neighbours a thread
+        constexpr int DIGITS = SORT_MAX_DIGITS / SORT_THREADS;
+        int c[DIGITS], h[DIGITS], sum = 0;
+#pragma unroll
+        for (int j = 0; j < DIGITS; ++j) {
+            const int d = threadIdx.x * DIGITS + j;
+            c[j] = d < digits ? a.totals[d] : 0;
+            h[j] = d < digits ? a.hist[(long long)d * blocks + blockIdx.x] : 0;
+            sum += c[j];
+        }
+        int incl = sum;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, incl, s);
-            if (lane >= s) incl += t;
+            const int v = __shfl_up_sync(0xffffffffu, incl, s);
+            if (lane >= s) incl += v;
         }
-        if (b < a.n_blocks) h[b] = run + incl - v;
-        run += __shfl_sync(0xffffffffu, incl, 31);
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        int run = incl - sum;
+        for (int w = 0; w < warp; ++w) run += s_sum[w];
+#pragma unroll
+        for (int j = 0; j < DIGITS; ++j) {
+            const int d = threadIdx.x * DIGITS + j;
+            if (d < digits) s_first[d] = run + h[j];
+            run += c[j];
+        }
+        if (pass == 0 && blockIdx.x == 0 && threadIdx.x == SORT_THREADS - 1) *a.count = run;
+        __syncthreads();
+
+        for (long long t = from; t < to; t += SORT_BLOCK) {  // (the same for the whole block)
+            uint32_t key[PER];
+            int place[PER], rank[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const long long i = t + warp * SORT_PER_WARP + j * 32 + lane;
+                key[j] = key_at(i);
+                place[j] = pass && i < to ? places_in[i] : (int)i;
+            }
+            for (int d = lane; d < digits; d += 32) s_warp[warp][d] = 0;
+            __syncwarp();
+            // rank within the warp, in order of position
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const bool ok = key[j] != NO_ROW;
+                // what is not there shares a digit no pair has, and so matches only its like
+                const int d = ok ? digit(key[j]) : SORT_MAX_DIGITS;
+                const unsigned peers = __match_any_sync(0xffffffffu, d);
+                const int before = __popc(peers & ((1u << lane) - 1u));
+                rank[j] = ok ? s_warp[warp][d] + before : 0;
+                __syncwarp();
+                if (ok && before == 0) s_warp[warp][d] += __popc(peers);
+                __syncwarp();
+            }
+            __syncthreads();
+            for (int d = threadIdx.x; d < digits; d += SORT_THREADS) {
+                int slot = s_first[d];
+#pragma unroll
+                for (int w = 0; w < SORT_WARPS; ++w) {
+                    const int n = s_warp[w][d];
+                    s_warp[w][d] = slot;
+                    slot += n;
+                }
+                s_first[d] = slot;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (key[j] == NO_ROW) continue;
+                const long long slot = s_warp[warp][digit(key[j])] + rank[j];
+                // slot < n by construction; the guard keeps a corrupted workspace from turning into a stray write
+                if (slot >= 0 && slot < a.n) {
+                    keys_out[slot] = key[j];
+                    places_out[slot] = place[j];
+                }
+            }
+            __syncthreads();
+        }
+        if (pass + 1 < a.passes) grid.sync();
     }
-    if (lane == 0) a.totals[d] = run;
-}
-
-// places of a block in order: warp w takes SORT_PER_WARP neighbours, 32 at a time
-__global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(SortArgs a) {
-    __shared__ int s_first[SORT_MAX_DIGITS];              // the block's first slot per digit
-    __shared__ int s_warp[SORT_WARPS][SORT_MAX_DIGITS];   // per warp: counts, then first slots
-    __shared__ int s_sum[SORT_WARPS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-
     let_next_start();
-    if (a.keys_in) wait_for_previous();  // (the first pass reads tokens before)
-    const long long count = a.keys_in ? *a.count_in : a.n;
-    const long long base = (long long)blockIdx.x * SORT_BLOCK + (long long)warp * SORT_PER_WARP;
-    uint32_t key[SORT_PER_WARP / 32];
-    int place[SORT_PER_WARP / 32], rank[SORT_PER_WARP / 32];
-#pragma unroll
-    for (int j = 0; j < SORT_PER_WARP / 32; ++j)
-        if (!sort_load(a, base + j * 32 + lane, count, key[j], place[j])) key[j] = NO_ROW;
-
-    if (!a.keys_in) wait_for_previous();
-
-    // first slot of every digit: exclusive sums of the totals, four digits a thread
-    constexpr int PER = SORT_MAX_DIGITS / SORT_THREADS;
-    int t[PER], h[PER], sum = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int d = threadIdx.x * PER + j;
-        t[j] = d < a.digits ? a.totals[d] : 0;
-        h[j] = d < a.digits ? a.hist[(long long)d * a.n_blocks + blockIdx.x] : 0;
-        sum += t[j];
-    }
-    int incl = sum;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, s);
-        if (lane >= s) incl += v;
-    }
-    if (lane == 31) s_sum[warp] = incl;
-    for (int d = lane; d < a.digits; d += 32) s_warp[warp][d] = 0;
-    __syncthreads();
-    int run = incl - sum;
-    for (int w = 0; w < warp; ++w) run += s_sum[w];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const int d = threadIdx.x * PER + j;
-        if (d < a.digits) s_first[d] = run + h[j];
-        run += t[j];
-    }
-    if (a.count_out && blockIdx.x == 0 && threadIdx.x == SORT_THREADS - 1) *a.count_out = run;
-
-    // rank within the warp, in order of place
-#pragma unroll
-    for (int j = 0; j < SORT_PER_WARP / 32; ++j) {
-        const bool ok = key[j] != NO_ROW;
-        // pairs that are not there share a digit no pair has, so they match only each other
-        const int d = ok ? (int)((key[j] >> a.shift) & (a.digits - 1)) : SORT_MAX_DIGITS;
-        const unsigned peers = __match_any_sync(0xffffffffu, d);
-        const int before = __popc(peers & ((1u << lane) - 1u));
-        rank[j] = ok ? s_warp[warp][d] + before : 0;
-        __syncwarp();
-        if (ok && before == 0) s_warp[warp][d] += __popc(peers);
-        __syncwarp();
-    }
-    __syncthreads();
-    for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) {
-        int slot = s_first[d];
-#pragma unroll
-        for (int w = 0; w < SORT_WARPS; ++w) {
-            const int c = s_warp[w][d];
-            s_warp[w][d] = slot;
-            slot += c;
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < SORT_PER_WARP / 32; ++j) {
-        if (key[j] == NO_ROW) continue;
-        const long long slot = s_warp[warp][(key[j] >> a.shift) & (a.digits - 1)] + rank[j];
-        // slot < n by construction; the guard keeps a corrupted workspace from turning into a stray write
-        if (slot >= 0 && slot < a.n) {
-            a.keys_out[slot] = key[j];
-            a.places_out[slot] = place[j];
-        }
-    }
 }
 
 // ---------------------------------------------------------------------------
@@ -666,7 +668,7 @@ static void launch_sums(SegmentArgs& a, cudaStream_t s) {
 // the call's plan and workspace: a pure function of the sizes and the device
 // ---------------------------------------------------------------------------
 struct EmbedPlan {
-    int passes, bits, n_blocks, chunks;
+    int passes, bits, blocks, chunks;
     size_t off_keys[2], off_places[2], off_hist, off_totals, off_count, off_part, bytes;
 };
 
@@ -676,7 +678,9 @@ static int plan_embed_grad(long long n, long long rows, long long D, int dtype, 
     while ((1ll << bits) < rows) ++bits;
     p->passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
     p->bits = (bits + p->passes - 1) / p->passes;
-    p->n_blocks = (int)((n + SORT_BLOCK - 1) / SORT_BLOCK);
+    // (at most one sorting block an SM: they wait for each other, and all fit the device at once)
+    const long long tiles = (n + SORT_BLOCK - 1) / SORT_BLOCK;
+    p->blocks = (int)(tiles < sm_count(device) ? tiles : sm_count(device));
     // One wave of blocks: 512 threads an SM, 16 bytes of columns a thread.
     const long long packs = (D * (long long)dtype_size(dtype) + 15) / 16, g = 1ll << group_log(packs);
     long long chunks = (long long)sm_count(device) * 512 / ((packs + g - 1) / g * g);
@@ -693,7 +697,7 @@ static int plan_embed_grad(long long n, long long rows, long long D, int dtype, 
         p->off_keys[i] = take((size_t)n * 4);
         p->off_places[i] = take((size_t)n * 4);
     }
-    p->off_hist = take((size_t)(1 << p->bits) * p->n_blocks * 4);
+    p->off_hist = take((size_t)(1 << p->bits) * p->blocks * 4);
     p->off_totals = take((size_t)(1 << p->bits) * 4);
     p->off_count = take(4);
     p->off_part = take((size_t)p->chunks * 2 * D * 4);
@@ -764,36 +768,31 @@ extern "C" int igs_embed_grad(const void* tokens, int token_bytes, long long n, 
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     SortArgs so{};
     so.tokens = Tokens{tokens, token_bytes == 8, has_empty != 0, empty, rows};
+    for (int i = 0; i < 2; ++i) {
+        so.keys[i] = reinterpret_cast<uint32_t*>(ws + p.off_keys[i]);
+        so.places[i] = reinterpret_cast<int*>(ws + p.off_places[i]);
+    }
     so.hist = reinterpret_cast<int*>(ws + p.off_hist);
     so.totals = reinterpret_cast<int*>(ws + p.off_totals);
-    int* count = reinterpret_cast<int*>(ws + p.off_count);
-    so.count_in = count;
+    so.count = reinterpret_cast<int*>(ws + p.off_count);
     so.n = n;
-    so.n_blocks = p.n_blocks;
-    so.digits = 1 << p.bits;
-    const int passes = n <= RANK_MAX ? 0 : p.passes;
-    if (!passes) {
-        so.keys_out = reinterpret_cast<uint32_t*>(ws + p.off_keys[0]);
-        so.places_out = reinterpret_cast<int*>(ws + p.off_places[0]);
-        so.count_out = count;
+    so.passes = p.passes;
+    so.bits = p.bits;
+    int sorted = 0;
+    if (n <= RANK_MAX) {
         sort_rank_kernel<<<(unsigned)((n + 31) / 32), RANK_WARPS * 32, 0, s>>>(so);
-        count_launch();
+    } else {
+        void* args[] = {&so};
+        const cudaError_t e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(sort_kernel), dim3((unsigned)p.blocks),
+                                                          dim3(SORT_THREADS), args, 0, s);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return (int)e;
+        }
+        sorted = (p.passes & 1) ^ 1;
     }
-    for (int pass = 0; pass < passes; ++pass) {
-        const int to = pass & 1;
-        so.keys_in = pass ? reinterpret_cast<uint32_t*>(ws + p.off_keys[to ^ 1]) : nullptr;
-        so.places_in = pass ? reinterpret_cast<int*>(ws + p.off_places[to ^ 1]) : nullptr;
-        so.keys_out = reinterpret_cast<uint32_t*>(ws + p.off_keys[to]);
-        so.places_out = reinterpret_cast<int*>(ws + p.off_places[to]);
-        so.count_out = pass ? nullptr : count;
-        so.shift = pass * p.bits;
-        if (!pass) sort_count_kernel<<<p.n_blocks, SORT_THREADS, 0, s>>>(so);
-        else launch_chained(sort_count_kernel, p.n_blocks, SORT_THREADS, 0, s, so);
-        launch_chained(sort_scan_kernel, (so.digits + SORT_WARPS - 1) / SORT_WARPS, SORT_THREADS, 0, s, so);
-        launch_chained(sort_place_kernel, p.n_blocks, SORT_THREADS, 0, s, so);
-        count_launch(3);
-    }
-    SegmentArgs a{so.keys_out, so.places_out, count, dy, d_table, reinterpret_cast<float*>(ws + p.off_part), rows, D,
+    count_launch();
+    SegmentArgs a{so.keys[sorted], so.places[sorted], so.count, dy, d_table, reinterpret_cast<float*>(ws + p.off_part), rows, D,
                   scale, p.chunks, 0, 0};
     const int bytes = embed_pack_bytes(dy, d_table, D, D, dtype_size(dtype));
     with_dtype(dtype, [&](auto t) {
