@@ -125,15 +125,17 @@ __global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(EmbedArgs a, int l
 template <typename T, int V>
 static void launch_embed(const EmbedArgs& a, int device, cudaStream_t s) {
     // Four loads in flight a thread (with two or eight 65536 rows of 1024 bf16 took 37 and 43 us instead of
-    // 35): over rows where a row has one pack a thread, within the row where it has more.  Rows go
-    // several to a group once that still leaves every SM sixteen blocks; below, latency counts.
+    // 35): of four rows where a row has one pack a thread, of two rows where it has more (four of one
+    // row: 41 instead of 31 us for 60000 rows of 514 bf16).  Rows go several to a group once that still
+    // leaves every SM sixteen blocks; below, latency counts.
     constexpr int MOST = 4;
     const int log_g = group_log(a.D / V);
     const long long groups = EMBED_THREADS >> log_g;
     const bool wide = a.D / V > EMBED_THREADS, many = a.n >= (long long)sm_count(device) * 16 * groups * MOST;
-    const long long per = groups * (many && !wide ? MOST : 1);
+    const long long per = groups * (!many ? 1 : wide ? 2 : MOST);
     const unsigned grid = (unsigned)((a.n + per - 1) / per);
-    if (wide) embed_kernel<T, V, 1, MOST><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
+    if (wide && many) embed_kernel<T, V, 2, 2><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
+    else if (wide) embed_kernel<T, V, 1, MOST><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
     else if (many) embed_kernel<T, V, MOST, 1><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
     else embed_kernel<T, V, 1, 1><<<grid, EMBED_THREADS, 0, s>>>(a, log_g);
 }
@@ -156,6 +158,10 @@ struct SortArgs {
 // before it, counted over all keys.  Block b ranks the places 32 b .. 32 b + 31, one a lane; each
 // warp counts over a share of the keys.  n^2 comparisons, but one launch and no passes: 8192 places
 // are 67 million comparisons, a few microseconds over the whole device.
+__device__ __forceinline__ void count_below(int& n, uint32_t key, uint32_t below) {
+    // (a predicated add; from `n += key < below` the compiler made five instructions)
+    asm("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %1, %2;\n\t@p add.s32 %0, %0, 1;\n\t}" : "+r"(n) : "r"(key), "r"(below));
+}
 constexpr int RANK_MAX = 8192;
 constexpr int RANK_WARPS = 16;
 __global__ void __launch_bounds__(RANK_WARPS * 32) sort_rank_kernel(SortArgs a) {
@@ -196,7 +202,10 @@ __global__ void __launch_bounds__(RANK_WARPS * 32) sort_rank_kernel(SortArgs a) 
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint4 k = tile[j];
-                rank += (k.x < below) + (k.y < below) + (k.z < below) + (k.w < below);
+                count_below(rank, k.x, below);
+                count_below(rank, k.y, below);
+                count_below(rank, k.z, below);
+                count_below(rank, k.w, below);
             }
         }
     }
@@ -221,8 +230,10 @@ __global__ void __launch_bounds__(RANK_WARPS * 32) sort_rank_kernel(SortArgs a) 
     }
 }
 
-// More places: all passes in one cooperative launch (three launches a pass took 19 us on the device for
-// 65536 places and two passes, this NEWTIME, and every launch costs the host 4).  Block b owns a range of
+// More places: all passes in one cooperative launch.  (Three chained launches a pass take 5 us less on
+// the device, 62 instead of 67 us for the whole gradient of 65536 places of width 1024 and two passes,
+// but every launch costs the host 4: forward and gradient of 9000 places of width 32 take 52 us this
+// way and 71 that.)  Block b owns a range of
 // neighbouring positions.  A pass: it counts the digits of its range; once all have, it finds from the
 // counts where each digit of its range goes (behind all smaller digits, and behind the same digit of
 // the blocks before); then it ranks its range in order, 32 positions a warp at a time, and writes the pairs.
