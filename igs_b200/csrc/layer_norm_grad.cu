@@ -363,7 +363,8 @@ extern "C" int igs_layer_norm_grad(const void* dy, const void* x, int dtype, lon
     const size_t wsize = dtype_size(wdtype);
     if (rows > 0 && (!dy || !x || !stats || !aligned_to(stats, 16))) return IGS_ERR_ARG;
     const bool columns = dweight || dbias;
-    if (rows > 0 && columns && (!workspace || workspace_bytes < igs_layer_norm_grad_workspace_bytes(rows, D, device)))
+    if (rows > 0 && columns &&
+        (!workspace || !aligned_to(workspace, 16) || workspace_bytes < igs_layer_norm_grad_workspace_bytes(rows, D, device)))
         return IGS_ERR_WORKSPACE;
     DeviceGuard guard(device);
     if (!guard.ok) return IGS_ERR_DEVICE;

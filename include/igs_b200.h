@@ -441,7 +441,8 @@ int igs_layer_norm(const void* x, int dtype, long long rows, long long D, long l
 /*
  * Its gradient: dx [rows,D] (contiguous, x's type), dweight and dbias [D] (wdtype), each NULL
  * when not wanted.  dy [rows,D] contiguous.  The column sums are taken over fixed blocks of
- * rows and added in a fixed order: the same bits on every call.
+ * rows and added in a fixed order: the same bits on every call.  The workspace (needed for the
+ * column sums) starts on a 16-byte boundary.
  */
 size_t igs_layer_norm_grad_workspace_bytes(long long rows, long long D, int device);
 int igs_layer_norm_grad(const void* dy, const void* x, int dtype, long long rows, long long D,

@@ -48,7 +48,7 @@ def test_c_abi_refuses_bad_arguments_before_any_cuda_call():
 
     for bad in (dict(tok=None), dict(dy=None), dict(out=None), dict(dt=-1), dict(rows=0), dict(scale=float("inf"))):
         assert embed_grad(**bad) == -1, bad
-    assert embed_grad(ws=None) == -2 and embed_grad(nb=16) == -2
+    assert embed_grad(ws=None) == -2 and embed_grad(nb=16) == -2 and embed_grad(ws=ctypes.c_void_p(264)) == -2
 
     def norm(x=one, dt=1, rows=4, D=8, stride=8, w=one, b=one, wdt=0, eps=1e-5, y=one, stats=one):
         return lib.igs_layer_norm(x, dt, rows, D, stride, w, b, wdt, eps, y, stats, 0, None)
@@ -63,7 +63,7 @@ def test_c_abi_refuses_bad_arguments_before_any_cuda_call():
 
     for bad in (dict(dy=None), dict(x=None), dict(stats=None), dict(stats=ctypes.c_void_p(260)), dict(wdt=2), dict(rows=-1)):
         assert norm_grad(**bad) == -1, bad
-    assert norm_grad(ws=None) == -2 and norm_grad(nb=16) == -2
+    assert norm_grad(ws=None) == -2 and norm_grad(nb=16) == -2 and norm_grad(ws=ctypes.c_void_p(264)) == -2
 
     def dropout(x=one, dt=0, n=4, p=0.5, y=one):
         return lib.igs_dropout(x, dt, n, p, 0, 0, None, y, 0, None)

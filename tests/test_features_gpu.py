@@ -445,6 +445,72 @@ def _passes(dev, seed, n=3000, rows=400, D=136, dtype=torch.bfloat16):
     return ins, run
 
 
+def test_differentiable_once(dev):
+    """A second derivative raises instead of passing for zero; so does a second backward pass."""
+    from igs_b200 import features
+
+    x = torch.randn(6, 16, device=dev, requires_grad=True)
+    w = torch.randn(16, device=dev, requires_grad=True)
+    tok = torch.tensor([0, 3, 3], device=dev)
+    for y, leaf in ((features.embed(tok, x), x), (features.layer_norm(x, w), w), (features.dropout(x, 0.5, 1), x)):
+        (g,) = torch.autograd.grad((y * y).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            g.sum().backward()
+    y = features.layer_norm(x, w)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    y = features.layer_norm(x, w)
+    with torch.no_grad():
+        x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_upstream_gradients_off_their_boundary(dev, dtype):
+    """Contiguous upstream gradients that start one value behind a 16-byte boundary."""
+    gen, t = _gen(dev, 31), ref.DTYPES[dtype]
+    shifted = lambda *shape: _normal(gen, int(np.prod(shape)) + 1, dtype=t)[1:].view(*shape)
+    _check_embed(torch.randint(0, 30, (90,), generator=gen, device=dev), _normal(gen, 30, 64, dtype=t), shifted(90, 64))
+    _check_norm(_normal(gen, 90, 64, dtype=t), _normal(gen, 64, dtype=t), _normal(gen, 64, dtype=t), shifted(90, 64))
+    _check_norm(shifted(1500, 64), _normal(gen, 64, dtype=t), _normal(gen, 64, dtype=t), _normal(gen, 1500, 64, dtype=t))
+    _check_dropout(_normal(gen, 90, 64, dtype=t), 0.3, 8, 9, shifted(90, 64), False)
+
+
+def test_first_calls_inside_a_capture():
+    """In a process of its own: nothing has to run before a capture (no call allocates, synchronises
+    or sets up in a way that a capture forbids)."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from igs_b200 import features
+dev = torch.device("cuda", 0)
+gen = torch.Generator(device=dev).manual_seed(0)
+tok = torch.randint(0, 500, (9000,), generator=gen, device=dev)
+table = torch.randn(500, 264, generator=gen, device=dev, requires_grad=True)
+w = torch.randn(264, generator=gen, device=dev, requires_grad=True)
+state = torch.tensor([1, 2], device=dev)
+def run():
+    f = features.layer_norm(features.embed(tok, table), w)
+    y = features.dropout(f, 0.5, state)
+    return (y, *torch.autograd.grad(y, (table, w), torch.ones_like(y)))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    outs = run()
+g.replay()
+for a, b in zip(outs, run()):
+    assert torch.equal(a, b)
+print("same")
+"""
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240,
+                         cwd=str(__import__("pathlib").Path(__file__).resolve().parents[1]))
+    assert res.returncode == 0 and "same" in res.stdout, res.stderr[-2000:]
+
+
 def test_same_bits_every_time(dev):
     ins, run = _passes(dev, 1, n=40000, rows=300)
     first = run(ins)
