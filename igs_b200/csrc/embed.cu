@@ -474,48 +474,44 @@ __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
     extern __shared__ __align__(16) unsigned char s_mem[];
     Pack<T, V>* ring = reinterpret_cast<Pack<T, V>*>(s_mem) + threadIdx.x;
     const auto slot = [&](int stage, int u, int i) { return ring + ((stage * CHUNK_STEP + u) * ITEMS + i) * EMBED_THREADS; };
-    const auto source = [&](int place, int i) {
-        return reinterpret_cast<const Pack<T, V>*>(dy + (long long)place * a.D) + i * g;
-    };
+    const auto source = [&](int place) { return reinterpret_cast<const Pack<T, V>*>(dy + (long long)place * a.D); };
 
     // Keys and places of a step (lo is a multiple of CHUNK_STEP and the sort's arrays are padded to 256
-    // bytes: whole packs; what lies behind hi is not used)
-    struct Step {
-        Pack<uint32_t, 4> key[CHUNK_STEP / 4];
-        Pack<int, 4> place[CHUNK_STEP / 4];
-    };
-    const auto load_step = [&](long long p, Step& s) {
-        if (p >= hi) return;
+    // bytes: whole packs; what lies behind hi is not used).  Steps: positions lo + i CHUNK_STEP.
+    const int length = (int)(hi - lo);
+    const uint32_t* keys = a.keys + lo;
+    const int* places = a.places + lo;
+    Pack<int, 4> place[CHUNK_STEP / 4];  // of the next step to fetch
+    const auto load_places = [&](int i) {
+        if (i * CHUNK_STEP >= length) return;
 #pragma unroll
-        for (int q = 0; q < CHUNK_STEP / 4; ++q) {
-            s.key[q] = reinterpret_cast<const Pack<uint32_t, 4>*>(a.keys + p)[q];
-            s.place[q] = reinterpret_cast<const Pack<int, 4>*>(a.places + p)[q];
-        }
+        for (int q = 0; q < CHUNK_STEP / 4; ++q) place[q] = reinterpret_cast<const Pack<int, 4>*>(places + i * CHUNK_STEP)[q];
     };
-    const auto fetch = [&](long long p, const Step& s, int stage) {
+    const auto fetch = [&](int i, int stage) {
+        const int n = length - i * CHUNK_STEP;
 #pragma unroll
         for (int u = 0; u < CHUNK_STEP; ++u) {
-            if (p + u >= hi) break;
+            if (u >= n) break;
+            const Pack<T, V>* row = source(place[u / 4].v[u % 4]);
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
-                if (i == 0 || i * g < mine) copy_async<sizeof(Pack<T, V>)>(slot(stage, u, i), source(s.place[u / 4].v[u % 4], i));
+            for (int k = 0; k < ITEMS; ++k)
+                if (k == 0 || k * g < mine) copy_async<sizeof(Pack<T, V>)>(slot(stage, u, k), row + k * g);
         }
     };
 
     // pipeline: step i is added while the rows of i + 1 and i + 2 are on their way and the places of
     // i + 3 are loaded
     static_assert(SEGMENT_STAGES == 3, "the pipeline below");
-    Step s0, s1, s2, s3;
-    load_step(lo, s0);
-    load_step(lo + CHUNK_STEP, s1);
-    load_step(lo + 2 * CHUNK_STEP, s2);
+    load_places(0);
     if constexpr (ASYNC) {
-        fetch(lo, s0, 0);
+        fetch(0, 0);
         copy_commit();
-        fetch(lo + CHUNK_STEP, s1, 1);
+        load_places(1);
+        fetch(1, 1);
         copy_commit();
+        load_places(2);
     }
-    uint32_t key = s0.key[0].v[0];
+    uint32_t key = keys[0];
     bool first = true;
     Vals<V> sum[ITEMS];
 #pragma unroll
@@ -533,40 +529,42 @@ __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
         first = false;
     };
     int stage = 0;
-    for (long long p = lo; p < hi; p += CHUNK_STEP) {
-        load_step(p + 3 * CHUNK_STEP, s3);
+    for (int i = 0; i * CHUNK_STEP < length; ++i) {
+        const int n = length - i * CHUNK_STEP;
+        Pack<uint32_t, 4> k[CHUNK_STEP / 4];
+#pragma unroll
+        for (int q = 0; q < CHUNK_STEP / 4; ++q) k[q] = reinterpret_cast<const Pack<uint32_t, 4>*>(keys + i * CHUNK_STEP)[q];
         Pack<T, V> v[CHUNK_STEP][ITEMS];
         if constexpr (ASYNC) {
-            fetch(p + 2 * CHUNK_STEP, s2, stage == 0 ? 2 : stage - 1);
+            fetch(i + 2, stage == 0 ? 2 : stage - 1);
             copy_commit();
+            load_places(i + 3);
             copy_wait<SEGMENT_STAGES - 1>();
         }
 #pragma unroll
         for (int u = 0; u < CHUNK_STEP; ++u) {
-            if (p + u >= hi) break;
+            if (u >= n) break;
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                if (i > 0 && i * g >= mine) break;
-                if constexpr (ASYNC) v[u][i] = *slot(stage, u, i);
-                else v[u][i] = *source(s0.place[u / 4].v[u % 4], i);
+            for (int j = 0; j < ITEMS; ++j) {
+                if (j > 0 && j * g >= mine) break;
+                if constexpr (ASYNC) v[u][j] = *slot(stage, u, j);
+                else v[u][j] = source(place[u / 4].v[u % 4])[j * g];
             }
         }
+        if constexpr (!ASYNC) load_places(i + 1);
         stage = stage == 2 ? 0 : stage + 1;
 #pragma unroll
         for (int u = 0; u < CHUNK_STEP; ++u) {
-            if (p + u >= hi) break;
-            const uint32_t ku = s0.key[u / 4].v[u % 4];
+            if (u >= n) break;
+            const uint32_t ku = k[u / 4].v[u % 4];
             if (ku != key) {  // (the same in every thread of the group)
                 finish_run(false);
                 key = ku;
             }
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i)
-                if (i == 0 || i * g < mine) sum[i] = add(sum[i], to_vals<T, V>(v[u][i]));
+            for (int j = 0; j < ITEMS; ++j)
+                if (j == 0 || j * g < mine) sum[j] = add(sum[j], to_vals<T, V>(v[u][j]));
         }
-        s0 = s1;
-        s1 = s2;
-        s2 = s3;
     }
     if constexpr (ASYNC) copy_wait<0>();
     finish_run(goes_on);
