@@ -59,6 +59,27 @@ def test_embed_sizes(dev, dtype, n, rows, D):
     _check_embed(tokens, _normal(gen, rows, D, dtype=t), _normal(gen, n, D, dtype=t), scale=1.7)
 
 
+@pytest.mark.parametrize("n,rows,D", [(70000, 300, 240), (17001, 5000, 1000), (33000, (1 << 20) + 9, 520)])
+def test_embed_many_places_of_wide_rows(dev, n, rows, D):
+    """The sort of many places in one, two and three passes, over wide rows; some places empty."""
+    gen = _gen(dev, n)
+    tokens = torch.randint(-1, rows, (n,), generator=gen, device=dev)
+    tokens[: n // 3] = tokens[0].clamp(min=0)  # a run over many chunks
+    from igs_b200 import features
+
+    table = torch.zeros(rows, D, device=dev, requires_grad=True)
+    dy = _normal(gen, n, D)
+    (g,) = torch.autograd.grad(features.embed(tokens, table, empty=-1), table, dy)
+    # the rows that have a token, in 64 bits on the device; all others are zero
+    held = tokens >= 0
+    uniq, at, times = torch.unique(tokens[held], return_inverse=True, return_counts=True)
+    want = torch.zeros(len(uniq), D, dtype=torch.float64, device=dev).index_add_(0, at, dy[held].double())
+    size = torch.zeros_like(want).index_add_(0, at, dy[held].double().abs())
+    assert ((g[uniq].double() - want).abs() <= 1.01 * ref.U * times[:, None] * size + 1e-40).all()
+    g[uniq] = 0
+    assert not g.any()
+
+
 @pytest.mark.parametrize("n", [40, 3000, 12000, 70000])
 @pytest.mark.parametrize("kind", ["one_token", "two_tokens", "first_and_last", "sorted", "reversed", "common"])
 def test_embed_token_patterns(dev, kind, n):
