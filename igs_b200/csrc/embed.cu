@@ -156,8 +156,8 @@ struct SortArgs {
 
 // Few places: every place's slot is the number of keys below its own plus the number of equal ones
 // before it, counted over all keys.  Block b ranks the places 32 b .. 32 b + 31, one a lane; each
-// warp counts over a share of the keys.  n^2 comparisons, but one launch and no passes: 8192 places
-// are 67 million comparisons, a few microseconds over the whole device.
+// warp counts over a share of the keys.  n^2 comparisons, but one launch and no passes: the 67 million
+// of 8192 places take about 12 us over the whole device, the passes below 20.
 __device__ __forceinline__ void count_below(int& n, uint32_t key, uint32_t below) {
     // (a predicated add; from `n += key < below` the compiler made five instructions)
     asm("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %1, %2;\n\t@p add.s32 %0, %0, 1;\n\t}" : "+r"(n) : "r"(key), "r"(below));
@@ -230,13 +230,13 @@ __global__ void __launch_bounds__(RANK_WARPS * 32) sort_rank_kernel(SortArgs a) 
     }
 }
 
-// More places: all passes in one cooperative launch.  (Three chained launches a pass take 5 us less on
-// the device, 62 instead of 67 us for the whole gradient of 65536 places of width 1024 and two passes,
-// but every launch costs the host 4: forward and gradient of 9000 places of width 32 take 52 us this
-// way and 71 that.)  Block b owns a range of
+// More places: all passes in one cooperative launch.  (Three chained launches a pass take 3 us less on
+// the device, 18 instead of 21 for 65536 places and two passes, but every launch costs the host 4: forward
+// and gradient of 9000 places of width 32 take 52 us this way and 71 that.)  Block b owns a range of
 // neighbouring positions.  A pass: it counts the digits of its range; once all have, it finds from the
 // counts where each digit of its range goes (behind all smaller digits, and behind the same digit of
-// the blocks before); then it ranks its range in order, 32 positions a warp at a time, and writes the pairs.
+// the blocks before); then it ranks its range in order, 32 positions a warp at a time, and writes the
+// pairs.
 __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
     __shared__ int s_first[SORT_MAX_DIGITS];             // counts, then the next slot per digit
     __shared__ int s_warp[SORT_WARPS][SORT_MAX_DIGITS];  // per warp: counts, then first slots

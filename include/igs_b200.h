@@ -9,7 +9,8 @@
  *
  * Conventions
  *   - every pointer is a DEVICE pointer on `device` unless stated otherwise; all
- *     tensors are fp32 and contiguous except x / y, which carry element strides;
+ *     tensors are fp32 and contiguous except x / y, which carry element strides, and what
+ *     the feature operators (at the end) say of theirs;
  *   - `stream` is a cudaStream_t passed as void*; nothing synchronises the stream
  *     except igs_read_status, igs_read_status_static,
  *     igs_read_executed and igs_profile_read;
