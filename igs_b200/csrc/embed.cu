@@ -80,7 +80,8 @@ struct EmbedArgs {
 };
 
 // A group of 2^log_g threads copies R rows, U packs of V values a thread at a time: the R tokens, then
-// R U independent loads in flight.
+// R U independent loads in flight.  Bound by memory and by how many rows are on their way: 65536 rows
+// of 1024 bf16 from a table of 16384 take 33 us, writing them alone 21.
 template <typename T, int V, int R, int U>
 __global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(EmbedArgs a, int log_g) {
     const int g = 1 << log_g, lane = threadIdx.x & (g - 1);
@@ -570,6 +571,7 @@ __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
     finish_run(goes_on);
 }
 
+// (6 us after the segments of 65536 places: latency, a handful of dependent loads.)
 // Runs that cross chunk borders: the tail of the chunk in which the run starts, then the heads of
 // the chunks that follow.  Q columns a thread.
 //   Short runs, up to JOIN_SHORT heads: in the first blocks `span` threads (whole warps) per chunk that

@@ -79,7 +79,9 @@ __global__ void __launch_bounds__(norm_block(G)) layer_norm_kernel(NormArgs a) {
 
 // Many rows: blocks stay and rows stream by, R at a time a group, so that the weights are read from
 // memory once a block, and each thread copies its packs of the next batches to shared memory of its own
-// ahead of time (cp.async), so that memory does not wait for a row's two sums.
+// ahead of time (cp.async), so that memory does not wait for a row's two sums.  Bound by memory: 65536
+// rows of 1024 bf16 take 48 us, a copy of them 43 (one group of registers a row, its weights read from L1
+// each time: 57, that pipe 96 % busy).
 template <typename T, typename W, int V, int G, int ITEMS, int FULL, int R>
 __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stream_kernel(NormArgs a) {
     constexpr int BLOCK = norm_block(G), GROUPS = BLOCK / G, PACK = sizeof(Pack<T, V>);
