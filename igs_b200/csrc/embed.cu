@@ -6,7 +6,8 @@
 // places of one token next to each other in their own order, so every row is one sum in 32 bits
 // with a fixed sequence and one rounding, the same bits on every run.
 //   1. sort.  Up to RANK_MAX places: one kernel ranks every place against all keys.  More: least
-//      significant digits first, up to 10 bits a pass (a codebook of a million rows needs two).
+//      significant digits first, up to 10 bits a pass (a codebook of a million rows needs two), or
+//      the whole row as one digit where its counts fit shared memory.
 //      Places without a token in the table drop out.
 //   2. segments: the sorted places are cut into chunks of equal length whatever the tokens are
 //      (one common token may own most of them).  A run of one token inside a chunk is finished
@@ -380,6 +381,119 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
     let_next_start();
 }
 
+// Codebooks of 1025 to 16384 rows and one tile a block: one pass, a digit being the whole row.  The
+// blocks' counts are [blocks][rows]; a thread per row sums its column over the blocks.  A block's 1024
+// pairs are ranked without any order between warps: an entry of 64 bits per row holds each warp's count
+// in a byte of its own (a warp has 128 pairs).  Whole gradient, two passes as above
+// against this: 27696 places of 5003 x 771 fp32 68 and 62 us, 65536 of 16384 x 1024 bf16 67 and 64, 131072
+// of 2000 x 64 57 and 49, 9000 of 16384 x 64 35 and 37.
+constexpr int WIDE_MAX_BITS = 14;
+__global__ void __launch_bounds__(SORT_THREADS) sort_wide_kernel(SortArgs a) {
+    extern __shared__ __align__(16) unsigned char s_mem[];
+    __shared__ int s_sum[SORT_WARPS], s_base[(1 << WIDE_MAX_BITS) / SORT_THREADS];
+    constexpr int PER = SORT_PER_WARP / 32;
+    static_assert(SORT_WARPS == 8 && SORT_PER_WARP < 256, "a byte a warp");
+    const auto grid = cooperative_groups::this_grid();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = (int)gridDim.x;
+    const int digits = 1 << a.bits;
+    int* s_count = reinterpret_cast<int*>(s_mem);                                  // [digits]
+    unsigned long long* s_ranks = reinterpret_cast<unsigned long long*>(s_mem);    // [digits], later
+    int* mine = a.hist + (long long)blockIdx.x * digits;                           // this block's counts, then first slots
+
+    const long long first = (long long)blockIdx.x * SORT_BLOCK + warp * SORT_PER_WARP + lane;
+    uint32_t key[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = first + j * 32 < a.n ? row_of(a.tokens, token_at(a.tokens, first + j * 32)) : NO_ROW;
+    for (int d = threadIdx.x; d < digits / 4; d += SORT_THREADS) reinterpret_cast<int4*>(s_count)[d] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        if (key[j] != NO_ROW) atomicAdd(&s_count[key[j]], 1);  // (integer counts: no order changes the result)
+    __syncthreads();
+    for (int d = threadIdx.x; d < digits / 4; d += SORT_THREADS) reinterpret_cast<int4*>(mine)[d] = reinterpret_cast<int4*>(s_count)[d];
+    grid.sync();
+
+    // a thread per row: exclusive sums over the blocks; then over the rows of a group of SORT_THREADS
+    int* group_sums = a.totals + digits;
+    for (int d0 = blockIdx.x * SORT_THREADS; d0 < digits; d0 += blocks * SORT_THREADS) {
+        int* column = a.hist + d0 + threadIdx.x;
+        int run = 0;
+        constexpr int U = 16;  // loads on their way together
+        for (int b0 = 0; b0 < blocks; b0 += U) {
+            int v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = b0 + u < blocks ? column[(long long)(b0 + u) * digits] : 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (b0 + u < blocks) column[(long long)(b0 + u) * digits] = run;
+                run += v[u];
+            }
+        }
+        int incl = run;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, incl, s);
+            if (lane >= s) incl += t;
+        }
+        if (lane == 31) s_sum[warp] = incl;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) incl += s_sum[w];
+        a.totals[d0 + threadIdx.x] = incl - run;
+        if (threadIdx.x == SORT_THREADS - 1) group_sums[d0 / SORT_THREADS] = incl;
+        __syncthreads();
+    }
+    grid.sync();
+
+    // where this block's pairs of a row go: behind the groups before, the rows before in the group, and
+    // the same row in the blocks before
+    int slot[PER], rank[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        slot[j] = key[j] != NO_ROW ? mine[key[j]] + a.totals[key[j]] : 0;
+        if (key[j] != NO_ROW) s_ranks[key[j]] = 0;
+    }
+    const int groups = digits / SORT_THREADS;
+    if (warp == 0) {
+        int run = 0;
+        for (int g0 = 0; g0 < groups; g0 += 32) {
+            const int v = g0 + lane < groups ? group_sums[g0 + lane] : 0;
+            int incl = v;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, incl, s);
+                if (lane >= s) incl += t;
+            }
+            if (g0 + lane < groups) s_base[g0 + lane] = run + incl - v;
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (blockIdx.x == 0 && lane == 0) *a.count = run;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const unsigned peers = __match_any_sync(0xffffffffu, key[j]);
+        const int before = __popc(peers & ((1u << lane) - 1u)), leader = __ffs(peers) - 1;
+        unsigned long long old = 0;
+        if (key[j] != NO_ROW && lane == leader) old = atomicAdd(&s_ranks[key[j]], (unsigned long long)__popc(peers) << (8 * warp));
+        old = __shfl_sync(0xffffffffu, old, leader);
+        rank[j] = (int)(old >> (8 * warp) & 255) + before;  // (only this warp adds to its byte)
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (key[j] == NO_ROW) continue;
+        const unsigned long long others = s_ranks[key[j]] & ((1ull << (8 * warp)) - 1);  // the warps before
+        const long long at = (long long)s_base[key[j] / SORT_THREADS] + slot[j] + rank[j] +
+                             __dp4a((unsigned)others, 0x01010101u, __dp4a((unsigned)(others >> 32), 0x01010101u, 0u));
+        // at < n by construction; the guard keeps a corrupted workspace from turning into a stray write
+        if (at >= 0 && at < a.n) {
+            a.keys[0][at] = key[j];
+            a.places[0][at] = (int)(first + j * 32);
+        }
+    }
+    let_next_start();
+}
+
 // ---------------------------------------------------------------------------
 // sums over runs of one token
 // ---------------------------------------------------------------------------
@@ -571,14 +685,14 @@ __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
     finish_run(goes_on);
 }
 
-// (6 us after the segments of 65536 places: latency, a handful of dependent loads.)
 // Runs that cross chunk borders: the tail of the chunk in which the run starts, then the heads of
 // the chunks that follow.  Q columns a thread.
 //   Short runs, up to JOIN_SHORT heads: in the first blocks `span` threads (whole warps) per chunk that
 //   may start one and slab of columns; a thread adds its columns up.
 //   Longer ones (they contain a chunk whose number is a multiple of JOIN_SHORT): one block per such
-//   chunk, which acts if it is the run's first.  32 threads across, 8 down: each of the 8 adds every
-//   8th row, and the 8 sums are added in order.
+//   chunk, which acts if it is the run's first.  32 threads across, 16 down: each of the 16 adds every
+//   16th row, and the 16 sums are added in order.
+// What bounds it is latency, a handful of dependent loads: 6 us behind the segments of 65536 places.
 constexpr int JOIN_SHORT = 16;
 constexpr int JOIN_THREADS = 512;
 constexpr int JOIN_DOWN = JOIN_THREADS / 32;
@@ -680,6 +794,7 @@ static void launch_sums(SegmentArgs& a, cudaStream_t s) {
 // ---------------------------------------------------------------------------
 struct EmbedPlan {
     int passes, bits, blocks, chunks;
+    bool wide;  // one pass, the digit being the row
     size_t off_keys[2], off_places[2], off_hist, off_totals, off_count, off_part, bytes;
 };
 
@@ -687,11 +802,12 @@ static int plan_embed_grad(long long n, long long rows, long long D, int dtype, 
     if (n > EMBED_MAX_PLACES || rows > EMBED_MAX_ROWS || D > EMBED_MAX_WIDTH) return IGS_ERR_LIMIT;
     int bits = 1;
     while ((1ll << bits) < rows) ++bits;
-    p->passes = (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
-    p->bits = (bits + p->passes - 1) / p->passes;
     // (at most one sorting block an SM: they wait for each other, and all fit the device at once)
     const long long tiles = (n + SORT_BLOCK - 1) / SORT_BLOCK;
     p->blocks = (int)(tiles < sm_count(device) ? tiles : sm_count(device));
+    p->wide = bits > SORT_MAX_BITS && bits <= WIDE_MAX_BITS && tiles == p->blocks;
+    p->passes = p->wide ? 1 : (bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
+    p->bits = (bits + p->passes - 1) / p->passes;
     // One wave of blocks: 512 threads an SM, 16 bytes of columns a thread.
     const long long packs = (D * (long long)dtype_size(dtype) + 15) / 16, g = 1ll << group_log(packs);
     long long chunks = (long long)sm_count(device) * 512 / ((packs + g - 1) / g * g);
@@ -709,11 +825,26 @@ static int plan_embed_grad(long long n, long long rows, long long D, int dtype, 
         p->off_places[i] = take((size_t)n * 4);
     }
     p->off_hist = take((size_t)(1 << p->bits) * p->blocks * 4);
-    p->off_totals = take((size_t)(1 << p->bits) * 4);
+    p->off_totals = take(((size_t)(1 << p->bits) + (1 << WIDE_MAX_BITS) / SORT_THREADS) * 4);
     p->off_count = take(4);
     p->off_part = take((size_t)p->chunks * 2 * D * 4);
     p->bytes = at;
     return IGS_OK;
+}
+
+// A cooperative launch of sorting blocks.
+static cudaError_t launch_waiting(void (*kernel)(SortArgs), size_t smem, SortArgs& a, int blocks, int device,
+                                  cudaStream_t s) {
+    static bool attr_set[64] = {};
+    if (smem > 48 * 1024 && (device < 0 || device >= 64 || !attr_set[device])) {
+        const cudaError_t e = cudaFuncSetAttribute(sort_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)(sizeof(unsigned long long) << WIDE_MAX_BITS));
+        if (e != cudaSuccess) return e;
+        if (device >= 0 && device < 64) attr_set[device] = true;
+    }
+    void* args[] = {&a};
+    return cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kernel), dim3((unsigned)blocks), dim3(SORT_THREADS), args,
+                                       smem, s);
 }
 
 static int token_args_ok(int token_bytes, long long n, long long rows, long long D, int dtype, float scale) {
@@ -793,9 +924,8 @@ extern "C" int igs_embed_grad(const void* tokens, int token_bytes, long long n, 
     if (n <= RANK_MAX) {
         sort_rank_kernel<<<(unsigned)((n + 31) / 32), RANK_WARPS * 32, 0, s>>>(so);
     } else {
-        void* args[] = {&so};
-        const cudaError_t e = cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(sort_kernel), dim3((unsigned)p.blocks),
-                                                          dim3(SORT_THREADS), args, 0, s);
+        const cudaError_t e = p.wide ? launch_waiting(sort_wide_kernel, sizeof(unsigned long long) << p.bits, so, p.blocks, device, s)
+                                     : launch_waiting(sort_kernel, 0, so, p.blocks, device, s);
         if (e != cudaSuccess) {
             cudaGetLastError();
             return (int)e;

@@ -51,7 +51,8 @@ def _check_embed(tokens, table, dy, scale=1.0, empty=None, what=""):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,rows,D", [
     (1, 1, 1), (1, 7, 1024), (2, 3, 5), (31, 2, 33), (33, 1000, 64), (257, 16, 129), (500, 501, 8), (1024, 300, 96),
-    (2047, 5, 40), (2049, 1030, 72), (4097, 70000, 24), (9001, 1 << 20, 3), (20011, 257, 17)])
+    (2047, 5, 40), (2049, 1030, 72), (4097, 70000, 24), (9001, 1 << 20, 3), (20011, 257, 17),
+    (9001, 16384, 9), (9500, 16385, 7), (8193, 1024, 6), (8193, 1025, 6), (151552, 1025, 4), (151553, 2048, 4)])
 def test_embed_sizes(dev, dtype, n, rows, D):
     gen = _gen(dev, n * 31 + D)
     t = ref.DTYPES[dtype]
