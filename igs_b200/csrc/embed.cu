@@ -383,22 +383,23 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
 
 // Codebooks of 1025 to 16384 rows and one tile a block: one pass, a digit being the whole row.  The
 // blocks' counts are [blocks][rows]; a thread per row sums its column over the blocks.  A block's 1024
-// pairs are ranked without any order between warps: an entry of 64 bits per row holds each warp's count
-// in a byte of its own (a warp has 128 pairs).  Whole gradient, two passes as above
-// against this: 27696 places of 5003 x 771 fp32 68 and 62 us, 65536 of 16384 x 1024 bf16 67 and 64, 131072
-// of 2000 x 64 57 and 49, 9000 of 16384 x 64 35 and 37.
+// pairs are ranked without any order between warps: an entry of 32 bits per row holds the counts of four
+// warps in a byte each (a warp has 128 pairs), first of warps 0 to 3, then of 4 to 7.  (64 bits would do it
+// in one round, 1 us sooner, but with 64 KB a block two calls' blocks fit an SM together.)  Whole gradient, two
+// passes as above against this: 27696 places of 5003 x 771 fp32 68 and 63 us, 65536 of 16384 x 1024 bf16
+// 67 and 65, 131072 of 2000 x 64 57 and 51, 9000 of 16384 x 64 35 and 37.
 constexpr int WIDE_MAX_BITS = 14;
 __global__ void __launch_bounds__(SORT_THREADS) sort_wide_kernel(SortArgs a) {
     extern __shared__ __align__(16) unsigned char s_mem[];
     __shared__ int s_sum[SORT_WARPS], s_base[(1 << WIDE_MAX_BITS) / SORT_THREADS];
     constexpr int PER = SORT_PER_WARP / 32;
-    static_assert(SORT_WARPS == 8 && SORT_PER_WARP < 256, "a byte a warp");
+    static_assert(SORT_WARPS == 8 && SORT_PER_WARP < 256, "a byte a warp, two rounds");
     const auto grid = cooperative_groups::this_grid();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = (int)gridDim.x;
     const int digits = 1 << a.bits;
-    int* s_count = reinterpret_cast<int*>(s_mem);                                  // [digits]
-    unsigned long long* s_ranks = reinterpret_cast<unsigned long long*>(s_mem);    // [digits], later
-    int* mine = a.hist + (long long)blockIdx.x * digits;                           // this block's counts, then first slots
+    int* s_count = reinterpret_cast<int*>(s_mem);            // [digits]
+    unsigned* s_ranks = reinterpret_cast<unsigned*>(s_mem);  // [digits], later
+    int* mine = a.hist + (long long)blockIdx.x * digits;     // this block's counts, then first slots
 
     const long long first = (long long)blockIdx.x * SORT_BLOCK + warp * SORT_PER_WARP + lane;
     uint32_t key[PER];
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_wide_kernel(SortArgs a) {
 
     // where this block's pairs of a row go: behind the groups before, the rows before in the group, and
     // the same row in the blocks before
-    int slot[PER], rank[PER];
+    int slot[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         slot[j] = key[j] != NO_ROW ? mine[key[j]] + a.totals[key[j]] : 0;
@@ -468,23 +469,40 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_wide_kernel(SortArgs a) {
         }
         if (blockIdx.x == 0 && lane == 0) *a.count = run;
     }
-    __syncthreads();
+    const int half = warp / 4, shift = 8 * (warp % 4);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        const unsigned peers = __match_any_sync(0xffffffffu, key[j]);
-        const int before = __popc(peers & ((1u << lane) - 1u)), leader = __ffs(peers) - 1;
-        unsigned long long old = 0;
-        if (key[j] != NO_ROW && lane == leader) old = atomicAdd(&s_ranks[key[j]], (unsigned long long)__popc(peers) << (8 * warp));
-        old = __shfl_sync(0xffffffffu, old, leader);
-        rank[j] = (int)(old >> (8 * warp) & 255) + before;  // (only this warp adds to its byte)
+    for (int round = 0; round < 2; ++round) {
+        __syncthreads();
+        if (half == round) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const unsigned peers = __match_any_sync(0xffffffffu, key[j]);
+                const int before = __popc(peers & ((1u << lane) - 1u)), leader = __ffs(peers) - 1;
+                unsigned old = 0;
+                if (key[j] != NO_ROW && lane == leader) old = atomicAdd(&s_ranks[key[j]], (unsigned)__popc(peers) << shift);
+                old = __shfl_sync(0xffffffffu, old, leader);
+                slot[j] += (int)(old >> shift & 255u) + before;  // (only this warp adds to its byte)
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (key[j] == NO_ROW || half < round) continue;
+            // the round's warps that come before this one
+            const unsigned counts = s_ranks[key[j]] & (half == round ? (1u << shift) - 1u : 0xffffffffu);
+            slot[j] += (int)__dp4a(counts, 0x01010101u, 0u);
+        }
+        if (round == 0) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (key[j] != NO_ROW) s_ranks[key[j]] = 0;
+        }
     }
-    __syncthreads();
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         if (key[j] == NO_ROW) continue;
-        const unsigned long long others = s_ranks[key[j]] & ((1ull << (8 * warp)) - 1);  // the warps before
-        const long long at = (long long)s_base[key[j] / SORT_THREADS] + slot[j] + rank[j] +
-                             __dp4a((unsigned)others, 0x01010101u, __dp4a((unsigned)(others >> 32), 0x01010101u, 0u));
+        const long long at = (long long)s_base[key[j] / SORT_THREADS] + slot[j];
         // at < n by construction; the guard keeps a corrupted workspace from turning into a stray write
         if (at >= 0 && at < a.n) {
             a.keys[0][at] = key[j];
@@ -838,7 +856,7 @@ static cudaError_t launch_waiting(void (*kernel)(SortArgs), size_t smem, SortArg
     static bool attr_set[64] = {};
     if (smem > 48 * 1024 && (device < 0 || device >= 64 || !attr_set[device])) {
         const cudaError_t e = cudaFuncSetAttribute(sort_wide_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)(sizeof(unsigned long long) << WIDE_MAX_BITS));
+                                                   (int)(sizeof(unsigned) << WIDE_MAX_BITS));
         if (e != cudaSuccess) return e;
         if (device >= 0 && device < 64) attr_set[device] = true;
     }
@@ -924,7 +942,7 @@ extern "C" int igs_embed_grad(const void* tokens, int token_bytes, long long n, 
     if (n <= RANK_MAX) {
         sort_rank_kernel<<<(unsigned)((n + 31) / 32), RANK_WARPS * 32, 0, s>>>(so);
     } else {
-        const cudaError_t e = p.wide ? launch_waiting(sort_wide_kernel, sizeof(unsigned long long) << p.bits, so, p.blocks, device, s)
+        const cudaError_t e = p.wide ? launch_waiting(sort_wide_kernel, sizeof(unsigned) << p.bits, so, p.blocks, device, s)
                                      : launch_waiting(sort_kernel, 0, so, p.blocks, device, s);
         if (e != cudaSuccess) {
             cudaGetLastError();

@@ -541,10 +541,12 @@ def test_same_bits_every_time(dev):
             assert torch.equal(a, b)
 
 
-def test_two_streams_at_once(dev):
-    """Two calls in flight on two streams, none of them the default one: each as on its own."""
-    ins1, run = _passes(dev, 2)
-    ins2, _ = _passes(dev, 3)
+@pytest.mark.parametrize("n,rows", [(3000, 400), (12000, 400), (12000, 5000)])
+def test_two_streams_at_once(dev, n, rows):
+    """Two calls in flight on two streams, none of them the default one: each as on its own.  (Every
+    kind of sort; blocks of two sorts that wait for their like fit the device together.)"""
+    ins1, run = _passes(dev, 2, n=n, rows=rows)
+    ins2, _ = _passes(dev, 3, n=n, rows=rows)
     want1, want2 = run(ins1), run(ins2)
     torch.cuda.synchronize()
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
