@@ -123,9 +123,12 @@ def prepare(case, seed):
 
     s = {"case": dict(case)}
     if case["op"] == "embed":
-        p = torch.from_numpy(_shares(case)).to(dev, torch.float32)
+        # (the running sum of the shares is taken on the host: on the GPU its last bits change from one
+        # call to the next, and with them a few of the tokens)
+        upto = torch.from_numpy(np.cumsum(_shares(case))).to(dev)
         n = case["batch"] * case["length"]
-        rank = torch.multinomial(p, n, replacement=True, generator=gen)
+        at = torch.rand(n, generator=gen, device=dev, dtype=torch.float64)
+        rank = torch.searchsorted(upto, at, right=True).clamp_(max=case["rows"] - 1)
         place = torch.randperm(case["rows"], generator=gen, device=dev)  # common tokens lie anywhere in the table
         tokens = place[rank].view(case["batch"], case["length"])
         if case["ragged"]:
