@@ -69,6 +69,23 @@ Tensor workspace(size_t bytes, const Tensor& like) {
     return at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, like.options().dtype(at::kByte));
 }
 
+// A tensor that comes back in a backward pass: the upstream gradient, or one that a saved-tensor hook
+// may have replaced (copied to another place, say).  Values are taken on trust, the layout is the
+// tensor's own, and what the kernels' addresses go by is checked.
+Tensor came_back(const char* name, Tensor t, at::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+    TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device, name,
+                " came back in the backward pass as another tensor than went in: expected ", type, " ", sizes, " on ", device,
+                t.defined() ? c10::str(", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device()) : ", got nothing");
+    return t;
+}
+
+// The upstream gradient of a node's only output, contiguous.
+Tensor upstream(const torch::autograd::Node& node, const Tensor& grad) {
+    const auto& out = node.input_metadata(0);
+    return came_back("the upstream gradient", grad, C10_AS_INTARRAYREF_SLOW(out.shape_as_dim_vector()),
+                     c10::typeMetaToScalarType(out.dtype()), out.device()).contiguous();
+}
+
 // What a backward pass under create_graph hands on: gradients that raise when they are
 // differentiated again, instead of passing for constants.
 variable_list once(variable_list grads) {
@@ -89,6 +106,8 @@ std::shared_ptr<N> make_node() {
 // embedding lookup
 // ---------------------------------------------------------------------------
 struct EmbedCall {
+    std::vector<int64_t> shape;  // of the tokens
+    at::ScalarType index = at::kLong;
     int64_t rows = 0, width = 0;
     float scale = 1;
     int has_empty = 0;
@@ -102,7 +121,8 @@ struct EmbedBackward : torch::autograd::Node {
     variable_list apply(variable_list&& grads) override {
         variable_list res(1);
         if (!grads[0].defined() || !task_should_compute_output(0)) return res;
-        const Tensor tokens = tokens_.unpack(), dy = grads[0].contiguous();
+        const Tensor dy = upstream(*this, grads[0]);
+        const Tensor tokens = came_back("tokens", tokens_.unpack(), call.shape, call.index, dy.device()).contiguous();
         const int64_t n = tokens.numel();
         Tensor d_table = at::empty({call.rows, call.width}, dy.options());
         size_t bytes = 0;
@@ -150,7 +170,9 @@ Tensor embed(const Tensor& tokens, const Tensor& table, double scale, std::optio
                         c.has_empty, c.empty, out.data_ptr(), device_index(tab), stream_of(tab)));
         if (grad) {
             node = make_node<EmbedBackward>();
-            node->call = c;
+            c.shape = tok.sizes().vec();
+            c.index = tok.scalar_type();
+            node->call = std::move(c);
             node->tokens_ = SavedVariable(tok, false);
         }
     }
@@ -192,13 +214,20 @@ bool as_rows(const Tensor& x, Rows& r) {
 struct NormBackward : torch::autograd::Node {
     SavedVariable x_, weight_;
     Tensor stats;  // [rows, 4]
-    Rows rows;
+    bool weighted;
     at::ScalarType wtype;
 
     variable_list apply(variable_list&& grads) override {
         variable_list res(3);
         if (!grads[0].defined()) return res;
-        const Tensor x = x_.unpack(), weight = weight_.unpack(), dy = grads[0].contiguous();
+        const Tensor dy = upstream(*this, grads[0]);
+        Tensor x = came_back("x", x_.unpack(), dy.sizes(), dy.scalar_type(), dy.device()), weight = weight_.unpack();
+        Rows rows;  // (of the tensor that came back)
+        if (!as_rows(x, rows)) {
+            x = x.contiguous();
+            as_rows(x, rows);
+        }
+        if (weighted) weight = came_back("weight", weight, {rows.width}, wtype, dy.device()).contiguous();
         const bool want_w = task_should_compute_output(1), want_b = task_should_compute_output(2);
         if (task_should_compute_output(0)) res[0] = at::empty(x.sizes(), dy.options());
         if (want_w) res[1] = at::empty({rows.width}, dy.options().dtype(wtype));
@@ -272,7 +301,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const s
             node->x_ = SavedVariable(src, false);
             node->weight_ = SavedVariable(w, false);
             node->stats = stats;
-            node->rows = r;
+            node->weighted = w.defined();
             node->wtype = wtype;
         }
     }
@@ -303,11 +332,14 @@ Tensor run_dropout(const Tensor& x, const DropoutCall& c, const Tensor& state) {
 struct DropoutBackward : torch::autograd::Node {
     SavedVariable state_;
     DropoutCall call;
+    bool stateful;
 
     variable_list apply(variable_list&& grads) override {
         variable_list res(1);
         if (!grads[0].defined() || !task_should_compute_output(0)) return res;
-        const Tensor state = state_.unpack(), dy = grads[0].contiguous();
+        const Tensor dy = upstream(*this, grads[0]);
+        Tensor state = state_.unpack();
+        if (stateful) state = came_back("seed", state, {2}, at::kLong, dy.device()).contiguous();
         res[0] = run_dropout(dy, call, state);
         return once(std::move(res));
     }
@@ -335,6 +367,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
         if (grad) {
             node = make_node<DropoutBackward>();
             node->call = call;
+            node->stateful = st.defined();
             node->state_ = SavedVariable(st, false);
         }
     }

@@ -1,0 +1,106 @@
+"""What reaches the feature operators other than by a plain call: tensors that come back changed in
+the backward pass, derivatives of other kinds, views whose values are not what lies in memory."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda", 0)
+
+
+def _calls(dev):
+    """{name: (leaves, function of them)}, the inputs strided, in several dimensions and in one"""
+    from igs_b200 import features
+
+    gen = torch.Generator(device=dev).manual_seed(3)
+    normal = lambda *s: torch.randn(s, generator=gen, device=dev)
+    wide, tokens = normal(30, 4, 200), torch.randint(-1, 30, (40, 3), generator=gen, device=dev)
+    w, b, state = normal(400)[::2], normal(200), torch.tensor([[5, 6], [7, 8]], device=dev)
+    leaf = lambda t: t.detach().requires_grad_()
+    calls = {}
+    for name, x in (("slice", wide[:, 1]), ("narrow", wide[:, 0, 8:136]), ("crossed", wide.transpose(0, 1)),
+                    ("columns", wide[:, 0].t().contiguous().t()), ("shared", wide[:1, 0].expand(7, 200)),
+                    ("one", wide[0, 0])):
+        D = x.shape[-1]
+        calls["norm " + name] = ([leaf(x), leaf(w[:D]), leaf(b[:D])], features.layer_norm)
+        calls["bare norm " + name] = ([leaf(x)], features.layer_norm)
+    calls["embed"] = ([leaf(wide[:, 2, 3:180])], lambda t: features.embed(tokens[:, 1:], t, empty=-1))
+    calls["dropout"] = ([leaf(wide[:, 1])], lambda x: features.dropout(x, 0.5, state[:, 0]))
+    calls["dropout by number"] = ([leaf(wide[:, 1])], lambda x: features.dropout(x, 0.5, 9))
+    return calls
+
+
+def _grads(leaves, fn):
+    y = fn(*leaves)
+    dy = torch.arange(y.numel(), device=y.device, dtype=y.dtype).view(y.shape).sin()
+    return torch.autograd.grad(y, leaves, dy)
+
+
+def _same(a, b):
+    assert len(a) == len(b) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+LAYOUTS = {
+    "contiguous": lambda t: t.clone(memory_format=torch.contiguous_format),
+    # (none of them moves a row off its 16-byte boundary: the kernels add in the same order)
+    "crossed": lambda t: t.permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim()))),
+    "spread": lambda t: torch.stack([t, t], -1)[..., 0],
+    "wider rows": lambda t: torch.cat([t, t], -1)[..., :t.shape[-1]],
+    "shifted": lambda t: torch.cat([t.new_zeros(4), t.reshape(-1)])[4:].view(t.shape),
+}
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_saved_tensors_come_back_in_another_layout(dev, layout):
+    """Gradients are the same bits wherever the saved tensors have been in between."""
+    for name, (leaves, fn) in _calls(dev).items():
+        want = _grads(leaves, fn)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, LAYOUTS[layout]):
+            _same(_grads(leaves, fn), want)
+
+
+def test_saved_tensors_kept_on_the_host(dev):
+    for pin in (False, True):
+        for name, (leaves, fn) in _calls(dev).items():
+            want = _grads(leaves, fn)
+            with torch.autograd.graph.save_on_cpu(pin_memory=pin):
+                _same(_grads(leaves, fn), want)
+
+
+def test_recomputed_forwards(dev):
+    from torch.utils.checkpoint import checkpoint
+
+    for name, (leaves, fn) in _calls(dev).items():
+        want = _grads(leaves, fn)
+        _same(_grads(leaves, lambda *a: checkpoint(fn, *a, use_reentrant=False)), want)
+
+
+@pytest.mark.parametrize("what", ["fewer", "more", "type", "place"])
+def test_other_tensors_that_come_back_are_refused(dev, what):
+    """A shorter, longer, retyped or host tensor: an error before anything is read."""
+    other = {"fewer": lambda t: t[:-1].clone(), "more": lambda t: torch.cat([t, t[:1]]),
+             "type": lambda t: t.to(torch.int32 if t.dtype == torch.int64 else torch.float64),
+             "place": lambda t: t.cpu()}[what]
+    for name, (leaves, fn) in _calls(dev).items():
+        if name == "dropout by number":
+            continue  # (nothing is saved)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+            y = fn(*leaves)
+            with pytest.raises(RuntimeError, match="came back in the backward pass"):
+                torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+
+def test_upstream_gradients_of_another_size_are_refused(dev):
+    """Handed to the node itself, past the checks of the engine."""
+    for name, (leaves, fn) in _calls(dev).items():
+        y = fn(*leaves)
+        for bad in (torch.ones(1, device=dev), torch.ones_like(y)[..., :-1], torch.ones_like(y).double(),
+                    torch.ones_like(y).cpu()):
+            with pytest.raises(RuntimeError, match="came back in the backward pass"):
+                y.grad_fn(bad)
+        got = y.grad_fn(torch.ones_like(y))  # (the right one, for the first time)
+        got = [got] if isinstance(got, torch.Tensor) else [g for g in got if g is not None]
+        _same(got, torch.autograd.grad(fn(*leaves).sum(), leaves))
