@@ -11,6 +11,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -45,9 +46,19 @@ int type_code(at::ScalarType t) {
     }
 }
 
+// These functions are not dispatched operators: torch would take their results for constants where it
+// looks for a tangent or records a trace.
+void refuse_forward_mode(const Tensor& t) {
+    TORCH_CHECK(!torch::autograd::isFwGradDefined(t), "the feature operators of igs_b200 have no forward-mode derivative");
+}
+void refuse_tracing() {
+    TORCH_CHECK(!torch::jit::tracer::isTracing(), "the feature operators of igs_b200 cannot be traced (torch.jit.trace)");
+}
+
 void require_features(const char* name, const Tensor& t) {
     TORCH_CHECK(t.is_cuda(), name, " is on ", t.device(), ": igs_b200 runs on CUDA devices only (no CPU path)");
     TORCH_CHECK_TYPE(type_code(t.scalar_type()) >= 0, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+    refuse_forward_mode(t);
 }
 
 void same_device(const char* name, const Tensor& t, const Tensor& first) {
@@ -82,6 +93,7 @@ Tensor came_back(const char* name, Tensor t, at::IntArrayRef sizes, at::ScalarTy
 // The upstream gradient of a node's only output, contiguous.
 Tensor upstream(const torch::autograd::Node& node, const Tensor& grad) {
     const auto& out = node.input_metadata(0);
+    refuse_forward_mode(grad);
     return came_back("the upstream gradient", grad, C10_AS_INTARRAYREF_SLOW(out.shape_as_dim_vector()),
                      c10::typeMetaToScalarType(out.dtype()), out.device()).contiguous();
 }
@@ -141,6 +153,7 @@ struct EmbedBackward : torch::autograd::Node {
 };
 
 Tensor embed(const Tensor& tokens, const Tensor& table, double scale, std::optional<int64_t> empty) {
+    refuse_tracing();
     require_features("table", table);
     TORCH_CHECK_TYPE(tokens.scalar_type() == at::kInt || tokens.scalar_type() == at::kLong,
                      "tokens must be int32 or int64, got ", tokens.scalar_type());
@@ -253,6 +266,7 @@ struct NormBackward : torch::autograd::Node {
 };
 
 Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps) {
+    refuse_tracing();
     require_features("x", x);
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, "x must be [...,D] with D >= 1, got ", x.sizes());
     const int64_t D = x.size(-1);
@@ -348,6 +362,7 @@ struct DropoutBackward : torch::autograd::Node {
 };
 
 Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const std::optional<Tensor>& state) {
+    refuse_tracing();
     require_features("x", x);
     TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "p must be in 0 .. 1, got ", p);
     if (state) {

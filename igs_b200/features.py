@@ -11,7 +11,8 @@ reference has no counterpart: its features are free parameters (scripts/gs2d_tes
 
 Like the splat they run on CUDA tensors only, on the current stream, asynchronously, and give
 the same bits on every call (no floating-point atomics).  Tensors are float32, bfloat16 or
-float16; everything is computed in 32 bits and rounded once.  Each is differentiable once.
+float16; everything is computed in 32 bits and rounded once.  Each is differentiable once, in
+reverse mode; forward-mode tangents, ``torch.func`` transforms and ``torch.jit.trace`` raise.
 """
 from __future__ import annotations
 

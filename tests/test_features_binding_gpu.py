@@ -104,3 +104,37 @@ def test_upstream_gradients_of_another_size_are_refused(dev):
         got = y.grad_fn(torch.ones_like(y))  # (the right one, for the first time)
         got = [got] if isinstance(got, torch.Tensor) else [g for g in got if g is not None]
         _same(got, torch.autograd.grad(fn(*leaves).sum(), leaves))
+
+
+def test_forward_mode_is_refused(dev):
+    """No operator has a forward-mode formula: an error, not a result whose tangent is lost."""
+    import torch.autograd.forward_ad as fwd
+
+    for name, (leaves, fn) in _calls(dev).items():
+        with fwd.dual_level():
+            for i in range(len(leaves)):
+                ins = [t.detach().clone() for t in leaves]  # (torch makes no dual of rows that share memory)
+                ins[i] = fwd.make_dual(ins[i], torch.ones_like(ins[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    fn(*ins)
+            y = fn(*leaves)
+            dy = fwd.make_dual(torch.ones_like(y), torch.ones_like(y))  # forward over reverse
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaves, dy)
+        _grads(leaves, fn)
+
+
+def test_transforms_are_refused(dev):
+    """Tracing would record the result as a constant; the others hand in tensors without memory."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    for name, (leaves, fn) in _calls(dev).items():
+        ins = [t.detach() for t in leaves]
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(fn, tuple(ins), check_trace=False)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(fn)(*[t.expand(2, *t.shape) for t in ins])
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda *a: fn(*a).sum())(*ins)
+        with pytest.raises(RuntimeError), FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            fn(*[mode.from_tensor(t) for t in ins])
