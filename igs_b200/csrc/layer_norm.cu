@@ -5,10 +5,14 @@
 //   g    = dy w,  dx = rstd (g - sum g / D - xhat sum(g xhat) / D)
 //   dw   = sum over rows of dy xhat,  db = sum over rows of dy
 //
-// All of it in 32 bits, one rounding per result.  The mean is kept as its distance `shift` from
-// the row's first value, mean = x[0] + shift: sums and differences of a row far from zero then
-// have the size of its spread, not of its distance from zero, and a constant row has variance 0
-// exactly.
+// All of it in 32 bits, one rounding per result, in two passes over a row's registers.  The first finds
+// a pivot, the mean up to rounding: x[0] plus the mean of x - x[0], which is x[0] itself in a constant
+// row.  The second sums c = x - pivot and c^2 together: mean = pivot + shift with shift = sum c / D, and
+// var = sum c^2 / D - shift^2.  Whatever the pivot's rounding was is in c and so in shift: rows far from
+// zero, and rows whose first value lies far from the others, keep what 32 bits can hold of their values'
+// distances from the mean, and a constant row has variance 0 exactly.  (With x - x[0] in place of x - pivot
+// in the second pass, the first pass's differences kept, N(0,1) rows whose first value is 1000 had a
+// relative error of 2e-5 in the others; now 1e-7.)
 //
 // No atomics: the column sums go through partial sums of fixed blocks of rows, which are added
 // in a fixed order.
@@ -30,7 +34,7 @@ struct NormArgs {
 // thread, held in registers between its one read and its one write.
 template <typename T, typename W, int V, int G, int ITEMS>
 __global__ void __launch_bounds__(norm_block(G)) layer_norm_kernel(NormArgs a) {
-    __shared__ float s_red[G > 32 ? 2 * (G / 32) : 1];
+    __shared__ __align__(16) float s_red[G > 32 ? 2 * (G / 32) * 2 : 1];
     const int lane = threadIdx.x % G;
     const float inv_d = 1.f / (float)a.D;
     const int packs = (int)(a.D / V);
@@ -49,31 +53,33 @@ __global__ void __launch_bounds__(norm_block(G)) layer_norm_kernel(NormArgs a) {
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         if (k * G >= mine) continue;
-        d[k] = sub(to_vals<T, V>(x[k]), splat<V>(x0));
-        sum = add(sum, d[k]);
+        d[k] = to_vals<T, V>(x[k]);
+        sum = add(sum, sub(d[k], splat<V>(x0)));
     }
-    float shift[1] = {total(sum)}, rstd[1];
-    group_sum<G, 1>(shift, s_red, 0);
-    shift[0] *= inv_d;
+    float first[1] = {total(sum)};
+    group_sum<G, 1>(first, s_red, 0);
+    const float pivot = fmaf(first[0], inv_d, x0);
+    Vals<V> sq = splat<V>(0.f);
     sum = splat<V>(0.f);
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         if (k * G >= mine) continue;
-        d[k] = sub(d[k], splat<V>(shift[0]));
-        sum = fma(d[k], d[k], sum);
+        d[k] = sub(d[k], splat<V>(pivot));
+        sum = add(sum, d[k]);
+        sq = fma(d[k], d[k], sq);
     }
-    rstd[0] = total(sum);
-    group_sum<G, 1>(rstd, s_red, 1);
-    rstd[0] = rsqrtf(rstd[0] * inv_d + a.eps);
+    float both[2] = {total(sum), total(sq)};
+    group_sum<G, 2>(both, s_red, 1);
+    const float shift = both[0] * inv_d, rstd = inverse_deviation(both[1] * inv_d, shift, a.eps);
     if (mine <= 0) return;
-    if (lane == 0 && a.stats) a.stats[row] = RowStats{x0, shift[0], rstd[0], 0.f};
+    if (lane == 0 && a.stats) a.stats[row] = RowStats{pivot, shift, rstd, 0.f};
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         if (k * G >= mine) continue;
         const int p = k * G + lane;
         const Vals<V> w = load_weights<W, V>(a.w, p, 1.f), b = load_weights<W, V>(a.b, p, 0.f);
         reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.D)[p] =
-            to_pack<T, V>(fma(mul(d[k], splat<V>(rstd[0])), w, b));
+            to_pack<T, V>(fma(fma(d[k], splat<V>(rstd), splat<V>(-shift * rstd)), w, b));
     }
 }
 
@@ -88,7 +94,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stre
     constexpr bool ASYNC = norm_async<T, V>;
     constexpr int STAGES = norm_stages<T, V>(ITEMS * R, BLOCK);
     extern __shared__ __align__(16) unsigned char s_mem[];
-    __shared__ float s_red[G > 32 ? 2 * (G / 32) * R : 1];
+    __shared__ __align__(16) float s_red[G > 32 ? 2 * (G / 32) * 2 * R : 1];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float inv_d = 1.f / (float)a.D;
     const int packs = (int)(a.D / V), mine = packs - lane;  // (item k is there when k G < mine)
@@ -153,7 +159,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stre
     for (int i = 0; i < steps; ++i) {
         const int left = i < steps - 1 ? R : tail;
         Vals<V> d[R][ITEMS];
-        float x0[R], shift[R], rstd[R];
+        float x0[R], pivot[R], both[2 * R];
         if constexpr (ASYNC) {
             fetch(stage == 0 ? STAGES - 1 : stage - 1);
             copy_commit();
@@ -175,32 +181,37 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stre
 #pragma unroll
             for (int k = 0; k < ITEMS; ++k) {
                 if (k >= FULL && k * G >= mine) continue;
-                d[r][k] = sub(to_vals<T, V>(x[k]), splat<V>(x0[r]));
-                sum = add(sum, d[r][k]);
+                d[r][k] = to_vals<T, V>(x[k]);
+                sum = add(sum, sub(d[r][k], splat<V>(x0[r])));
             }
-            shift[r] = total(sum);
+            pivot[r] = total(sum);
         }
         now += step * x_row;
         fetch_first(i + 1);
         stage = stage + 1 == STAGES ? 0 : stage + 1;
-        group_sum<G, R>(shift, s_red, 0);
+        group_sum<G, R>(pivot, s_red, 0);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            shift[r] *= inv_d;
-            Vals<V> sq = splat<V>(0.f);
+            pivot[r] = fmaf(pivot[r], inv_d, x0[r]);
+            Vals<V> sum = splat<V>(0.f), sq = splat<V>(0.f);
 #pragma unroll
             for (int k = 0; k < ITEMS; ++k) {
                 if (k >= FULL && k * G >= mine) continue;
-                d[r][k] = sub(d[r][k], splat<V>(shift[r]));
+                d[r][k] = sub(d[r][k], splat<V>(pivot[r]));
+                sum = add(sum, d[r][k]);
                 sq = fma(d[r][k], d[r][k], sq);
             }
-            rstd[r] = total(sq);
+            both[2 * r] = total(sum);
+            both[2 * r + 1] = total(sq);
         }
-        group_sum<G, R>(rstd, s_red, 1);
+        group_sum<G, 2 * R>(both, s_red, 1);
+        float rstd[R], offset[R];  // xhat = d rstd + offset
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            rstd[r] = rsqrtf(rstd[r] * inv_d + a.eps);
-            if (lane == 0 && stats && r < left) stats[r] = RowStats{x0[r], shift[r], rstd[r], 0.f};
+            const float shift = both[2 * r] * inv_d;
+            rstd[r] = inverse_deviation(both[2 * r + 1] * inv_d, shift, a.eps);
+            offset[r] = -shift * rstd[r];
+            if (lane == 0 && stats && r < left) stats[r] = RowStats{pivot[r], shift, rstd[r], 0.f};
         }
         if (stats) stats += step;
 #pragma unroll
@@ -211,17 +222,18 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stre
             for (int r = 0; r < R; ++r)
                 if (r < left)
                     *reinterpret_cast<Pack<T, V>*>(out + r * y_row + k * (G * PACK)) =
-                        to_pack<T, V>(fma(mul(d[r][k], splat<V>(rstd[r])), w, b));
+                        to_pack<T, V>(fma(fma(d[r][k], splat<V>(rstd[r]), splat<V>(offset[r])), w, b));
         }
         out += step * y_row;
     }
     if constexpr (ASYNC) copy_wait<0>();
 }
 
-// Rows of any width: one CTA per row, the row read three times (from L2 after the first).
+// Rows of any width: one CTA per row, the row read three times (from L2 after the first), eight CTAs an
+// SM to have enough of them on their way (1024 rows of 20000 fp32: 68 us, with six 92).
 template <typename T, typename W>
-__global__ void __launch_bounds__(LN_THREADS) layer_norm_any_kernel(NormArgs a) {
-    __shared__ float s_red[LN_RED];
+__global__ void __launch_bounds__(LN_THREADS, 8) layer_norm_any_kernel(NormArgs a) {
+    __shared__ __align__(16) float s_red[LN_RED];
     const W* w = static_cast<const W*>(a.w);
     const W* b = static_cast<const W*>(a.b);
     const float inv_d = 1.f / (float)a.D;
@@ -231,18 +243,21 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_any_kernel(NormArgs a) 
         const float x0 = to_f(x[0]);
         float sum = 0.f;
         for (long long c = threadIdx.x; c < a.D; c += LN_THREADS) sum += to_f(x[c]) - x0;
-        const float shift = block_sum_all(sum, s_red, 0) * inv_d;
-        float sq = 0.f;
+        const float pivot = fmaf(block_sum_all(sum, s_red, 0), inv_d, x0);
+        float sum_d = 0.f, sum_sq = 0.f;
         for (long long c = threadIdx.x; c < a.D; c += LN_THREADS) {
-            const float d = (to_f(x[c]) - x0) - shift;
-            sq = fmaf(d, d, sq);
+            const float d = to_f(x[c]) - pivot;
+            sum_d += d;
+            sum_sq = fmaf(d, d, sum_sq);
         }
-        const float rstd = rsqrtf(block_sum_all(sq, s_red, 1) * inv_d + a.eps);
+        float both[2] = {sum_d, sum_sq};
+        group_sum<LN_THREADS, 2>(both, s_red, 1);
+        const float shift = both[0] * inv_d, rstd = inverse_deviation(both[1] * inv_d, shift, a.eps), offset = -shift * rstd;
         for (long long c = threadIdx.x; c < a.D; c += LN_THREADS) {
-            const float xhat = ((to_f(x[c]) - x0) - shift) * rstd;
+            const float xhat = fmaf(to_f(x[c]) - pivot, rstd, offset);
             y[c] = from_f<T>(fmaf(xhat, w ? to_f(w[c]) : 1.f, b ? to_f(b[c]) : 0.f));
         }
-        if (threadIdx.x == 0 && a.stats) a.stats[r] = RowStats{x0, shift, rstd, 0.f};
+        if (threadIdx.x == 0 && a.stats) a.stats[r] = RowStats{pivot, shift, rstd, 0.f};
     }
 }
 

@@ -5,10 +5,18 @@
 
 namespace igs {
 
-// What the gradient needs of a row, one 16-byte load: its first value, mean - first value, rstd.
+// What the gradient needs of a row, one 16-byte load: its pivot, mean - pivot, rstd.
 struct alignas(16) RowStats {
-    float x0, shift, rstd, unused;
+    float pivot, shift, rstd, unused;
 };
+
+// 1 / sqrt(var + eps) from the mean of the squared distances from the pivot and the mean's own distance
+// `shift` from it.  The subtraction takes off at most half in rows that the type can tell from constant
+// ones; it is a fused one, so that an infinite mean square stays what it is.  (NaN passes the comparison.)
+__device__ __forceinline__ float inverse_deviation(float mean_square, float shift, float eps) {
+    const float var = fmaf(-shift, shift, mean_square);
+    return rsqrtf((var < 0.f ? 0.f : var) + eps);
+}
 
 // V weights; without any, the value they stand for
 template <typename W, int V>
@@ -22,8 +30,8 @@ __host__ __device__ constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_
 
 // N sums (a power of two, at most 32) over the G threads of a row's group at once, the same bits in
 // every one of them.  Groups of up to a warp are lanes of one warp; a wider group is the whole
-// block, and s_red (two halves used in turn, so that one barrier a call suffices) holds N floats
-// per warp.  Within a warp the first log2 N steps halve the number of sums a lane carries: N - 1
+// block, and s_red (on a 16-byte boundary; two halves used in turn, so that one barrier a call suffices)
+// holds N floats per warp.  Within a warp the first log2 N steps halve the number of sums a lane carries: N - 1
 // exchanges and 5 - log2 N more, instead of 5 N.
 template <int G, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* s_red, int turn) {
@@ -57,12 +65,17 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* s_red, int turn)
             float* red = s_red + turn * (WARPS * N);
             if ((lane & ((1 << SHIFT) - 1)) == 0) red[(threadIdx.x >> 5) * N + (lane >> SHIFT)] = v[0];
             __syncthreads();
+            constexpr int Q = N < 4 ? N : 4;  // sums that one load reads
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                float t = 0.f;
+            for (int i = 0; i < N; ++i) v[i] = 0.f;
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w) t += red[w * N + i];
-                v[i] = t;
+            for (int w = 0; w < WARPS; ++w) {
+#pragma unroll
+                for (int q = 0; q < N / Q; ++q) {
+                    const Pack<float, Q> t = reinterpret_cast<const Pack<float, Q>*>(red + w * N)[q];
+#pragma unroll
+                    for (int i = 0; i < Q; ++i) v[q * Q + i] += t.v[i];
+                }
             }
         }
     }
@@ -195,6 +208,6 @@ __device__ __forceinline__ float block_sum_all(float v, float* s_red, int turn) 
     group_sum<LN_THREADS, 1>(t, s_red, turn);
     return t[0];
 }
-constexpr int LN_RED = 2 * (LN_THREADS / 32);
+constexpr int LN_RED = 2 * 2 * (LN_THREADS / 32);  // (for two sums at once)
 
 }  // namespace igs

@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
     constexpr bool ASYNC = norm_async<T, V>;
     constexpr int STAGES = norm_stages<T, V>(2 * ITEMS * R, BLOCK);
     extern __shared__ __align__(16) unsigned char s_mem[];
-    __shared__ float s_red[G > 32 ? 2 * (G / 32) * 2 * R : 1];
+    __shared__ __align__(16) float s_red[G > 32 ? 2 * (G / 32) * 2 * R : 1];
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const float inv_d = 1.f / (float)a.D;
     const int packs = (int)(a.D / V), mine = packs - lane;  // (item k is there when k G < mine)
@@ -112,12 +112,12 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
             copy_commit();
             copy_wait<STAGES - 1>();
         }
-        Vals<V> s1[R], s2[R], x0[R], f[R], t[R];
+        Vals<V> s1[R], s2[R], pivot[R], f[R], t[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             rstd[r] = next[r].rstd;
             s1[r] = s2[r] = splat<V>(0.f);
-            x0[r] = splat<V>(next[r].x0);  // xhat = (x - x0) rstd - shift rstd
+            pivot[r] = splat<V>(next[r].pivot);  // xhat = (x - pivot) rstd - shift rstd
             f[r] = splat<V>(rstd[r]);
             t[r] = splat<V>(-next[r].shift * rstd[r]);
         }
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
                     pd = *reinterpret_cast<const Pack<T, V>*>(dy_now + r * y_row + k * (G * PACK));
                 }
                 const Vals<V> d = to_vals<T, V>(pd);
-                xh[r][k] = fma(sub(to_vals<T, V>(px), x0[r]), f[r], t[r]);
+                xh[r][k] = fma(sub(to_vals<T, V>(px), pivot[r]), f[r], t[r]);
                 g[r][k] = mul(d, w);
                 s1[r] = add(s1[r], g[r][k]);
                 s2[r] = fma(g[r][k], xh[r][k], s2[r]);
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_grad
 // Rows of any width, first part: one CTA per row, the row read twice (from L2 the second time).
 template <typename T, typename W>
 __global__ void __launch_bounds__(LN_THREADS) layer_norm_dx_any_kernel(NormGradArgs a) {
-    __shared__ float s_red[LN_RED];
+    __shared__ __align__(16) float s_red[LN_RED];
     const W* w = static_cast<const W*>(a.w);
     const float inv_d = 1.f / (float)a.D;
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -223,13 +223,13 @@ __global__ void __launch_bounds__(LN_THREADS) layer_norm_dx_any_kernel(NormGradA
         for (long long c = threadIdx.x; c < a.D; c += LN_THREADS) {
             const float g = to_f(dy[c]) * (w ? to_f(w[c]) : 1.f);
             s1 += g;
-            s2 = fmaf(g, ((to_f(x[c]) - st.x0) - st.shift) * st.rstd, s2);
+            s2 = fmaf(g, ((to_f(x[c]) - st.pivot) - st.shift) * st.rstd, s2);
         }
         const float m1 = block_sum_all(s1, s_red, 0) * inv_d;
         const float m2 = block_sum_all(s2, s_red, 1) * inv_d;
         for (long long c = threadIdx.x; c < a.D; c += LN_THREADS) {
             const float g = to_f(dy[c]) * (w ? to_f(w[c]) : 1.f);
-            dx[c] = from_f<T>(st.rstd * (g - m1 - ((to_f(x[c]) - st.x0) - st.shift) * st.rstd * m2));
+            dx[c] = from_f<T>(st.rstd * (g - m1 - ((to_f(x[c]) - st.pivot) - st.shift) * st.rstd * m2));
         }
     }
 }
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(32 * LN_COL_ROWS) layer_norm_columns_kernel(No
         for (long long r = lo + threadIdx.y; r < hi; r += LN_COL_ROWS) {
             const float dy = to_f(static_cast<const T*>(a.dy)[r * a.D + c]);
             const RowStats st = a.stats[r];
-            sw = fmaf(dy, ((to_f(static_cast<const T*>(a.x)[r * a.row_stride + c]) - st.x0) - st.shift) * st.rstd, sw);
+            sw = fmaf(dy, ((to_f(static_cast<const T*>(a.x)[r * a.row_stride + c]) - st.pivot) - st.shift) * st.rstd, sw);
             sb += dy;
         }
     }

@@ -432,8 +432,9 @@ int igs_embed_grad(const void* tokens, int token_bytes, long long n, const void*
  * 1 / sqrt(var + eps) with the biased variance.  x [rows,D] with `row_stride` elements between
  * rows, y [rows,D] contiguous; weight, bias [D] of type wdtype (x's type or IGS_F32) or NULL
  * for ones / zeros.  stats [rows,4] (fp32, on a 16-byte boundary) is what the gradient needs of
- * every row, NULL when it is not wanted: x[0], mean - x[0], rstd and a spare.  The mean is kept as
- * its distance from the row's first value so that rows far from zero lose nothing.
+ * every row, NULL when it is not wanted: a pivot (the mean up to rounding), mean - pivot, rstd and a
+ * spare.  Values are taken as distances from the pivot, and the pivot's own rounding is corrected for:
+ * neither rows far from zero nor rows with a few far values lose what 32 bits can hold of the others.
  */
 int igs_layer_norm(const void* x, int dtype, long long rows, long long D, long long row_stride,
                    const void* weight, const void* bias, int wdtype, float eps, void* y, float* stats,
