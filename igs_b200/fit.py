@@ -374,7 +374,8 @@ def fit_progressive(model, target, steps, lr=1e-4, chunk=4, ratios=(1 / 16, 1 / 
     (scripts/gs2d_test.py:154-189): every step draws a fraction of the features, renders
     only those, and steps AdamW on ``reconstruction + reg_weight * koleo(features[:k])``
     (of the codebook's rows for a model with tokens) with the gradient norm clipped to
-    ``clip``.  The reconstruction term is L1 + 0.5 MSE
+    ``clip``.  Any model will do that has ``num_features``, ``feature`` [1,N,D] (or
+    ``diverse(k)`` in its place) and the call of ``ProgressiveSplatter``.  The reconstruction term is L1 + 0.5 MSE
     (:53-60 without its MS-SSIM term, whose package is not available here).  Returns
     (losses [steps], the k of every step) on the CPU."""
     from .reg import koleo_diversity_loss
@@ -394,7 +395,8 @@ def fit_progressive(model, target, steps, lr=1e-4, chunk=4, ratios=(1 / 16, 1 / 
         ks.append(k)
         out, _ = model(num_active_features=k, size=size)
         recon = F.l1_loss(out, target) + 0.5 * mse_loss(out, target)
-        loss = recon + reg_weight * koleo_diversity_loss(model.diverse(k))
+        spread = model.diverse(k) if hasattr(model, "diverse") else model.feature[:, :k]
+        loss = recon + reg_weight * koleo_diversity_loss(spread)
         opt.zero_grad(set_to_none=True)
         loss.backward()
         torch.nn.utils.clip_grad_norm_(model.parameters(), clip)
