@@ -76,6 +76,9 @@ void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.devi
 int device_index(const Tensor& t) { return t.device().index(); }
 void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// The tensor with its values in its memory: torch keeps the sign of some views beside it.
+Tensor in_memory(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 Tensor workspace(size_t bytes, const Tensor& like) {
     return at::empty({static_cast<int64_t>(bytes < 256 ? 256 : bytes)}, like.options().dtype(at::kByte));
 }
@@ -87,7 +90,7 @@ Tensor came_back(const char* name, Tensor t, at::IntArrayRef sizes, at::ScalarTy
     TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device, name,
                 " came back in the backward pass as another tensor than went in: expected ", type, " ", sizes, " on ", device,
                 t.defined() ? c10::str(", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device()) : ", got nothing");
-    return t;
+    return in_memory(t);
 }
 
 // The upstream gradient of a node's only output, contiguous.
@@ -172,8 +175,9 @@ Tensor embed(const Tensor& tokens, const Tensor& table, double scale, std::optio
     Tensor out;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor tok = tokens.contiguous();
-        const Tensor tab = table.stride(1) == 1 || c.width == 1 ? table : table.contiguous();
+        const Tensor tok = in_memory(tokens).contiguous();
+        Tensor tab = in_memory(table);
+        if (tab.stride(1) != 1 && c.width != 1) tab = tab.contiguous();
         auto shape = tokens.sizes().vec();
         shape.push_back(c.width);
         out = at::empty(shape, table.options());
@@ -296,13 +300,13 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight_, const s
     {
         at::AutoDispatchBelowADInplaceOrView below;
         Rows r;
-        Tensor src = x;
-        if (!as_rows(x, r)) {
-            src = x.contiguous();
+        Tensor src = in_memory(x);
+        if (!as_rows(src, r)) {
+            src = src.contiguous();
             as_rows(src, r);
         }
-        const Tensor w = given[0].defined() ? given[0].contiguous() : Tensor();
-        const Tensor b = given[1].defined() ? given[1].contiguous() : Tensor();
+        const Tensor w = given[0].defined() ? in_memory(given[0]).contiguous() : Tensor();
+        const Tensor b = given[1].defined() ? in_memory(given[1]).contiguous() : Tensor();
         y = at::empty(x.sizes(), x.options());
         Tensor stats;
         if (grad) stats = at::empty({r.count, 4}, x.options().dtype(at::kFloat));
@@ -377,8 +381,8 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
     Tensor y;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor st = state ? state->contiguous() : Tensor();
-        y = run_dropout(x.contiguous(), call, st);
+        const Tensor st = state ? in_memory(*state).contiguous() : Tensor();
+        y = run_dropout(in_memory(x).contiguous(), call, st);
         if (grad) {
             node = make_node<DropoutBackward>();
             node->call = call;

@@ -138,3 +138,27 @@ def test_transforms_are_refused(dev):
             torch.func.grad(lambda *a: fn(*a).sum())(*ins)
         with pytest.raises(RuntimeError), FakeTensorMode(allow_non_fake_inputs=True) as mode:
             fn(*[mode.from_tensor(t) for t in ins])
+
+
+def test_negated_views(dev):
+    """Real tensors whose sign torch keeps beside the memory (imaginary parts of conjugates)."""
+    from igs_b200 import features
+
+    gen = torch.Generator(device=dev).manual_seed(8)
+    z = torch.complex(*(torch.randn(40, 1, generator=gen, device=dev) for _ in range(2)))
+    column, tokens = z.conj().imag, torch.randint(0, 40, (9,), generator=gen, device=dev)
+    wide = torch._neg_view(torch.randn(40, 24, generator=gen, device=dev))
+    dy = torch._neg_view(torch.randn(40, 24, generator=gen, device=dev))
+    assert column.is_neg() and wide.is_neg() and dy.is_neg()
+    vec, bias = torch._neg_view(wide[0].clone()), column[:1, 0]
+    plain = lambda t: t.clone().resolve_neg()
+    for fn, ins, up in ((lambda t: features.embed(tokens, t), [column], None), (lambda t: features.embed(tokens, t), [wide], None),
+                        (lambda t: features.dropout(t, 0.5, 3), [column[0]], None),
+                        (lambda t: features.dropout(t, 0.5, 3), [wide], dy),
+                        (lambda *t: features.layer_norm(*t), [wide, vec, vec], dy),
+                        (lambda *t: features.layer_norm(*t), [column, bias, bias], None)):
+        want_y = fn(*[plain(t) for t in ins])
+        assert torch.equal(fn(*ins), want_y)
+        up = torch.ones_like(want_y) if up is None else up
+        leaves, want_leaves = [t.detach().requires_grad_() for t in ins], [plain(t).requires_grad_() for t in ins]
+        _same(torch.autograd.grad(fn(*leaves), leaves, up), torch.autograd.grad(fn(*want_leaves), want_leaves, plain(up)))
