@@ -296,6 +296,9 @@ def fit(model, target, steps, lr=1e-2, graph=True, schedule=None, betas=(0.9, 0.
 # ---------------------------------------------------------------------------
 # feature -> image experiment with a random number of active features per step
 # ---------------------------------------------------------------------------
+DIVERSE_ROWS = 4096  # the diversity term is quadratic in them: 64 MB a matrix
+
+
 class ProgressiveSplatter(nn.Module):
     """Learned feature vectors rendered through the module, coarse to fine: the image of the
     first k features must already resemble the target (the reference's
@@ -361,8 +364,20 @@ class ProgressiveSplatter(nn.Module):
 
     def diverse(self, k):
         """[1,N,feature_dim]: the learned vectors that the diversity term of ``fit_progressive``
-        spreads, the first k features or the codebook's rows."""
-        return self.codebook[None] if hasattr(self, "codebook") else self.feature[:, :k]
+        spreads: the first k features, or the codebook's rows.  Of a codebook of more than
+        ``DIVERSE_ROWS`` rows those that the first k features of the images use, and at most
+        ``DIVERSE_ROWS`` of them, drawn anew by torch's generator (a gather that waits for the
+        device: how many there are decides what is launched)."""
+        if not hasattr(self, "codebook"):
+            return self.feature[:, :k]
+        if self.codebook.shape[0] <= DIVERSE_ROWS:
+            return self.codebook[None]
+        from . import features as ops
+
+        used = torch.unique(self.tokens[:, :k])
+        if used.numel() > DIVERSE_ROWS:
+            used = used[torch.randperm(used.numel(), device=used.device)[:DIVERSE_ROWS]]
+        return ops.embed(used, self.codebook)[None]
 
     def forward(self, num_active_features=None, size=None):
         return self.gs(self.features(num_active_features), size)
@@ -373,7 +388,7 @@ def fit_progressive(model, target, steps, lr=1e-4, chunk=4, ratios=(1 / 16, 1 / 
     """The training loop of the reference's feature -> image experiment
     (scripts/gs2d_test.py:154-189): every step draws a fraction of the features, renders
     only those, and steps AdamW on ``reconstruction + reg_weight * koleo(features[:k])``
-    (of the codebook's rows for a model with tokens) with the gradient norm clipped to
+    (of a model with tokens: the codebook's rows, see ``diverse``) with the gradient norm clipped to
     ``clip``.  Any model will do that has ``num_features``, ``feature`` [1,N,D] (or
     ``diverse(k)`` in its place) and the call of ``ProgressiveSplatter``.  The reconstruction term is L1 + 0.5 MSE
     (:53-60 without its MS-SSIM term, whose package is not available here).  Returns
