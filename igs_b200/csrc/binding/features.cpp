@@ -4,8 +4,8 @@
 // Why this is C++ while the splat's autograd Functions are Python: a splat takes hundreds of
 // microseconds on the device, these operators on the features of one image a few, and a Python
 // autograd Function with its ctypes call costs more than the kernels.  Forward and gradient of a
-// 128 x 1024 layer norm, issued from Python: 131 us that way; what torch's engine takes by itself
-// for an empty function of three inputs: 65 us.
+// 128 x 1024 layer norm, issued back to back: 131 us that way, 69 this way; torch's own negation of one
+// such tensor and its gradient take 50 on the same host.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>

@@ -82,7 +82,7 @@ struct EmbedArgs {
 
 // A group of 2^log_g threads copies R rows, U packs of V values a thread at a time: the R tokens, then
 // R U independent loads in flight.  Bound by memory and by how many rows are on their way: 65536 rows
-// of 1024 bf16 from a table of 16384 take 33 us, writing them alone 21.
+// of 1024 bf16 from a table of 16384 take 32 us, its bytes at a copy's rate 26.
 template <typename T, int V, int R, int U>
 __global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(EmbedArgs a, int log_g) {
     const int g = 1 << log_g, lane = threadIdx.x & (g - 1);
@@ -126,9 +126,9 @@ __global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(EmbedArgs a, int l
 
 template <typename T, int V>
 static void launch_embed(const EmbedArgs& a, int device, cudaStream_t s) {
-    // Four loads in flight a thread (with two or eight 65536 rows of 1024 bf16 took 37 and 43 us instead of
-    // 35): of four rows where a row has one pack a thread, of two rows where it has more (four of one
-    // row: 41 instead of 31 us for 60000 rows of 514 bf16).  Rows go several to a group once that still
+    // Four loads in flight a thread (with two or eight 65536 rows of 1024 bf16 took 6 and 23 % longer): of
+    // four rows where a row has one pack a thread, of two rows where it has more (four of one row: 60000
+    // rows of 514 bf16 took a third longer).  Rows go several to a group once that still
     // leaves every SM sixteen blocks; below, latency counts.
     constexpr int MOST = 4;
     const int log_g = group_log(a.D / V);
@@ -385,8 +385,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(SortArgs a) {
 // blocks' counts are [blocks][rows]; a thread per row sums its column over the blocks.  A block's 1024
 // pairs are ranked without any order between warps: an entry of 32 bits per row holds the counts of four
 // warps in a byte each (a warp has 128 pairs), first of warps 0 to 3, then of 4 to 7.  (64 bits would do it
-// in one round, 1 us sooner, but with 64 KB a block two calls' blocks fit an SM together.)  Whole gradient, two
-// passes as above against this: 27696 places of 5003 x 771 fp32 68 and 63 us, 65536 of 16384 x 1024 bf16
+// in one round, 1 us sooner, but with 64 KB a block two calls' blocks fit an SM together.)  Whole gradient
+// issued eagerly, two passes as above against this: 27696 places of 5003 x 771 fp32 68 and 63 us, 65536 of 16384 x 1024 bf16
 // 67 and 65, 131072 of 2000 x 64 57 and 51, 9000 of 16384 x 64 35 and 37.
 constexpr int WIDE_MAX_BITS = 14;
 __global__ void __launch_bounds__(SORT_THREADS) sort_wide_kernel(SortArgs a) {
@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(EMBED_THREADS) segment_kernel(SegmentArgs a) {
 //   Longer ones (they contain a chunk whose number is a multiple of JOIN_SHORT): one block per such
 //   chunk, which acts if it is the run's first.  32 threads across, 16 down: each of the 16 adds every
 //   16th row, and the 16 sums are added in order.
-// What bounds it is latency, a handful of dependent loads: 6 us behind the segments of 65536 places.
+// What bounds it is latency, a handful of dependent loads: 5 us behind the segments of 65536 places.
 constexpr int JOIN_SHORT = 16;
 constexpr int JOIN_THREADS = 512;
 constexpr int JOIN_DOWN = JOIN_THREADS / 32;

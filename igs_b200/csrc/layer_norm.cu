@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(norm_block(G)) layer_norm_kernel(NormArgs a) {
 
 // Many rows: blocks stay and rows stream by, R at a time a group, so that the weights are read from
 // memory once a block, and each thread copies its packs of the next batches to shared memory of its own
-// ahead of time (cp.async), so that memory does not wait for a row's two sums.  Bound by memory: 65536
-// rows of 1024 bf16 take 48 us, a copy of them 43 (one group of registers a row, its weights read from L1
+// ahead of time (cp.async), so that memory does not wait for a row's sums.  Bound by memory: 65536
+// rows of 1024 bf16 take 46 us, a copy of them 43 (one group of registers a row, its weights read from L1
 // each time: 57, that pipe 96 % busy).
 template <typename T, typename W, int V, int G, int ITEMS, int FULL, int R>
 __global__ void __launch_bounds__(norm_block(G), norm_blocks(G)) layer_norm_stream_kernel(NormArgs a) {
@@ -280,11 +280,11 @@ static bool with_norm_group(long long packs, F&& f) {
 template <typename T, typename W, int V>
 static bool launch_norm_packs(const NormArgs& a, int device, cudaStream_t s) {
     // Rows stream once every SM has several to keep its blocks busy; below, one group a row answers sooner
-    // (128 x 1024 fp32: 3.2 us instead of 6.4).
+    // (128 x 1024 fp32: 2.5 us, half of what streaming took).
     if (a.rows >= 8ll * sm_count(device)) {
         const bool done = with_stream_group<T, V>(a.D / V, [&](auto g, auto items, auto full) {
             constexpr int G = decltype(g)::value, ITEMS = decltype(items)::value, FULL = decltype(full)::value;
-            constexpr int R = G >= 256 ? 2 : ITEMS * V <= 16 ? 4 : 2;  // 64 values a thread in registers
+            constexpr int R = G >= 256 ? 2 : ITEMS * V <= 16 ? 4 : 2;  // 64 values a thread (few spill)
             constexpr int BLOCK = norm_block(G), PER = BLOCK / G * R;
             constexpr size_t ring = norm_async<T, V> ? sizeof(Pack<T, V>) * norm_stages<T, V>(ITEMS * R, BLOCK) * R * ITEMS * BLOCK : 0;
             constexpr size_t most = ring + (size_t)BLOCK / (BLOCK / G) * ITEMS * V * 2 * sizeof(float);  // (of the widest row)

@@ -5,8 +5,8 @@
 // [rows, D] (x, dy, dx), about 13 instructions a value.  A row's two sums need every thread of its
 // group between its loads and its stores; so that memory does not wait for them, each thread copies
 // its packs of the next rows to shared memory of its own ahead of time (cp.async; no thread reads
-// another's, no barrier is needed for it).  65536 rows of 1024 bf16: 71 us, and 4 for the column sums'
-// second step; the sum of two such tensors, the same traffic, takes 62.
+// another's, no barrier is needed for it).  65536 rows of 1024 bf16: 72 us with the column sums'
+// second step; the sum of two such tensors, the same traffic, takes 59.
 #include "layer_norm.cuh"
 
 namespace igs {
@@ -304,7 +304,9 @@ template <typename T, typename W, int V>
 static bool launch_norm_grad_packs(NormGradArgs& a, int device, cudaStream_t s) {
     return with_stream_group<T, V>(a.D / V, [&](auto g, auto items, auto full) {
         constexpr int G = decltype(g)::value, ITEMS = decltype(items)::value, FULL = decltype(full)::value;
-        constexpr int R = G >= 512 ? 1 : ITEMS * V <= 8 ? 4 : ITEMS * V <= 16 ? 2 : 1;  // 64 values a thread in registers, xhat and dy w
+        constexpr int R = G >= 512 ? 1 : ITEMS * V <= 8 ? 4 : ITEMS * V <= 16 ? 2 : 1;
+        // (64 values a thread, xhat and dy w; a fifth of the instances, all of 16-bit types, spill up to
+        // 152 bytes of them)
         constexpr int BLOCK = norm_block(G), PER = BLOCK / G * R;
         constexpr size_t ring = norm_async<T, V> ? sizeof(Pack<T, V>) * norm_stages<T, V>(2 * ITEMS * R, BLOCK) * R * 2 * ITEMS * BLOCK : 0;
         constexpr size_t cols = BLOCK > G ? (size_t)BLOCK * ITEMS * V * 2 * sizeof(float) : 0;

@@ -313,7 +313,8 @@ class ProgressiveSplatter(nn.Module):
     * ``norm``: a layer norm with learned weight and bias on every feature vector.
     * ``dropout``: the share of feature values that a training forward sets to zero.  Its
       generator's state (seed, offset) is a buffer on the device that every such forward moves on
-      by one, also when a captured graph replays it.
+      by one, also when a captured graph replays it.  (A forward that is run again for its backward
+      pass, as activation checkpointing does, would draw another mask: keep the features out of it.)
     """
 
     def __init__(self, num_features, feature_dim, gaussians_per_feature, channels=3, *, tokens=None, rows=None,
